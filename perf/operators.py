@@ -88,8 +88,7 @@ def work(case):
     B = case["batch"]
     if case["op"] == "append":
         n = B * case["tokens"]
-        old = int(_lengths(case).remainder(PAGE).sum()) * 2 * hkv * d           # tokens of the open pages, read and written
-        return dict(bytes=n * (2 * H + 2 * hkv) * d * size + n * d * 4 + 2 * n * hkv * d + 2 * old, flops=n * (H + 2 * hkv) * d * 3)
+        return dict(bytes=n * (2 * H + 2 * hkv) * d * size + n * d * 4 + 2 * n * hkv * d, flops=n * (H + 2 * hkv) * d * 3)
     if case["op"] == "attention":
         n = int(_lengths(case).sum())
         return dict(bytes=n * 2 * hkv * (d + 1) + B * 2 * H * d * size, flops=4 * n * H * d)
