@@ -48,7 +48,8 @@ typedef enum {
 
 typedef enum {
   TSB200_KV_INT8 = 0, TSB200_KV_FP8 = 1, TSB200_KV_NVFP4 = 2,
-  TSB200_KV_F32 = 3, TSB200_KV_BF16 = 4   /* unquantized pages in the act dtype */
+  TSB200_KV_F32 = 3, TSB200_KV_BF16 = 4,  /* unquantized pages in the act dtype */
+  TSB200_KV_FP8_PAGE = 5                  /* e4m3 pages, one scale per page and head   */
 } tsb200_kv_format;
 
 const char* tsb200_strerror(int status);
@@ -218,6 +219,11 @@ int tsb200_norm_mlp_gated(const tsb200_norm_desc* norm, const tsb200_linear_desc
  *   V fp8   : codes [d][16]
  *   V nvfp4 : codes [d/2][16] (byte = elements 2i | 2i+1<<4 of one token), scales [d/16][16]
  *   K, V f32 / bf16 (unquantized): values [16][d] in the act dtype
+ *   K fp8_page : codes [16][d]  (e4m3), then 16 bytes: the fp32 scale of the page and head, 12 bytes unused
+ *   V fp8_page : codes [d][16], then the same
+ * fp8_page: the scale is 2^e, e the smallest integer with amax <= 448 * 2^e over the finite elements of the page's tokens, -40 <= e <= 40.  Tokens
+ * appended to a page that holds others raise it where they need to (the older codes are then re-encoded) and never lower it; larger values
+ * saturate.  Nothing beside the pages belongs to the cache, so that sequences can share pages and tokens come one by one.
  * Pools must be zero-filled once when allocated: slots of a page beyond the sequence length
  * are read (and masked) by the attention kernels and must hold finite bit patterns.
  * ---------------------------------------------------------------------------------- */
@@ -264,6 +270,8 @@ int tsb200_kv_fp8_scales_strided(const void* k, const void* v, int dtype, int64_
  * appended as given).  Rotation is the half-split form of blocks/rope.py:140-173 with
  * each product and sum rounded to the act dtype.  seq_lens is NOT modified.
  * Positions beyond the block table (>= bt_stride*16) are skipped.
+ * fp8_page: the rotation is computed in fp32 (each product and sum rounded once) and k goes straight into its code, q is rounded once; slots
+ * of a page behind the sequence's new end become zero; the rope tables must be 16-byte aligned.
  * k/v_token_stride: elements between consecutive tokens (0 = hkv*d, i.e. dense), so k and v
  * may be column slices of one fused [B*T, (H + 2 hkv) d] projection output. */
 int tsb200_kv_append(const tsb200_kv_desc* kv, const void* k, const void* v, int dtype,
@@ -283,6 +291,29 @@ int tsb200_rope_append(const tsb200_kv_desc* kv, void* q, int q_heads, int64_t q
                        int64_t B, int64_t T, const int32_t* new_lens,
                        const float* rope_cos, const float* rope_sin, int64_t rope_rows,
                        void* stream);
+
+/* Beam search's reordering of a paged cache: row r of a batch of `rows` sequences takes over the cached tokens of row parents[r], in all
+ * `n_pools` pools (device array of device pointers to uint8 [num_pages, page_bytes]: K and V of every layer; page_bytes = hkv * record bytes) that
+ * share one block table.  Full pages become shared: block_table[r][0 .. seq_lens[r] / 16) is the parent's.  The entries from there on are the row's own
+ * and do not change; the page at seq_lens[r] / 16, where it holds tokens, gets the parent's bytes.  So that no row ever writes a page of another one, a
+ * block table starts with pages of its own for every row, and is put back to them before a sequence is started anew.
+ * A row whose parent is itself, is out of range, or has another length keeps what it has.  scales (may be NULL): device array of n_scales device
+ * pointers to fp32 [rows, scale_width], whose rows follow their parents too.  parents may name a row several times.  rows <= 2048.
+ * With tsb200_set_pdl on, the first append or attention after this call must be at least the second launch after it. */
+int tsb200_kv_reorder(void* const* pools, int n_pools, int64_t page_bytes, int64_t num_pages, float* const* scales, int n_scales,
+                      int scale_width, int32_t* block_table, int64_t bt_stride, const int32_t* seq_lens, const int32_t* parents, int64_t rows,
+                      void* stream);
+
+/* Beam search's selection.  logits [B * K, V] (rows row_stride elements apart, 0 = V), scores fp32 [B, K]: over the K * V continuations of a
+ * sequence, value = scores[k] + logits[k][t] - logsumexp(logits[k]), computed in 64 bits from fp32 exponentials; the n largest, in order, ties to the
+ * lowest k * V + t.  out_scores fp32, out_parents int32 (b * K + k: the row, as tsb200_kv_reorder takes it), out_tokens int64: [B, n].
+ * finished (may be NULL): bytes [B, K]; a finished beam has one continuation, pad_token at its own score.  A beam whose score is -infinity or not a
+ * number, or whose logits hold a NaN or +infinity, has none.  Where fewer than n values are above -infinity, the others are the lowest k * V + t left.
+ * n <= 32, n <= K * V, K <= 256. */
+size_t tsb200_beam_select_workspace_bytes(int64_t B, int K, int64_t V, int dtype, int n);
+int tsb200_beam_select(const void* logits, int dtype, int64_t row_stride, int64_t B, int K, int64_t V, const float* scores,
+                       const uint8_t* finished, int64_t pad_token, int n, float* out_scores, int32_t* out_parents, int64_t* out_tokens,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* Dequantizing gather: k_out, v_out [B, L, hkv, d] (act dtype) <- the first L positions of every
  * sequence, dequantized (fp8: times the sequence's scale); positions >= seq_lens[b] become zeros.

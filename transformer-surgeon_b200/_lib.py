@@ -11,7 +11,7 @@ LIB_PATH = os.path.join(_HERE, "libtsb200.so")
 
 OK, ERR_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_DEVICE, ERR_TIMEOUT = 0, -1, -2, -3, -4, -5, -6
 F32, BF16 = 0, 1
-KV_INT8, KV_FP8, KV_NVFP4, KV_F32, KV_BF16 = 0, 1, 2, 3, 4
+KV_INT8, KV_FP8, KV_NVFP4, KV_F32, KV_BF16, KV_FP8_PAGE = 0, 1, 2, 3, 4, 5
 KV_FRESH = 1
 
 
@@ -85,6 +85,9 @@ SIGNATURES = {
     "tsb200_paged_decode_attn_simt": (_i32, [_KD, _vp, _vp, _i32, _i64, _i64, _i32, _f32, _i64, _vp, _sz, _vp]),
     "tsb200_paged_decode_attn_static_capacity": (_sz, []),
     "tsb200_paged_decode_attn_static": (_i32, [_KD, _vp, _vp, _i32, _i64, _i64, _i32, _f32, _i64, _vp]),
+    "tsb200_kv_reorder": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _i32, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "tsb200_beam_select_workspace_bytes": (_sz, [_i64, _i32, _i64, _i32, _i32]),
+    "tsb200_beam_select": (_i32, [_vp, _i32, _i64, _i64, _i32, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
     "tsb200_rope": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
     "tsb200_peer_flag_bytes": (_sz, []),
     "tsb200_enable_peer_access": (_i32, [_i32]),

@@ -29,7 +29,7 @@ from . import ops
 from .decoder import CompressedDecoder, DecoderConfig, LayerWeights, fuse_rows
 
 # cache_impl values served here (the reference's own three stay with the reference)
-CACHE_IMPLS = ("paged_int8", "paged_fp8", "paged_nvfp4", "paged_bf16", "paged_fp32")
+CACHE_IMPLS = ("paged_int8", "paged_fp8", "paged_nvfp4", "paged_bf16", "paged_fp32", "paged_fp8_page")
 _BLOCK_LINEARS = ("attn.q_proj", "attn.k_proj", "attn.v_proj", "attn.out_proj", "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")
 
 

@@ -88,6 +88,7 @@ __device__ __forceinline__ float dense_elem(const uint8_t* __restrict__ rec, int
 }
 template <int D>
 __device__ __forceinline__ float k_elem(const uint8_t* __restrict__ rec, int fmt, int t, int e) {
+  if (fmt == TSB200_KV_FP8_PAGE) return e4m3_byte_to_f32(rec[t * D + e]) * *reinterpret_cast<const float*>(rec + 16 * D);
   if (fmt >= TSB200_KV_F32) return dense_elem<D>(rec, fmt, t, e);
   if (fmt == TSB200_KV_INT8)
     return (float)(int8_t)rec[t * D + e] * reinterpret_cast<const float*>(rec + 16 * D)[t];
@@ -97,6 +98,7 @@ __device__ __forceinline__ float k_elem(const uint8_t* __restrict__ rec, int fmt
 }
 template <int D>
 __device__ __forceinline__ float v_elem(const uint8_t* __restrict__ rec, int fmt, int t, int e) {
+  if (fmt == TSB200_KV_FP8_PAGE) return e4m3_byte_to_f32(rec[e * 16 + t]) * *reinterpret_cast<const float*>(rec + 16 * D);
   if (fmt >= TSB200_KV_F32) return dense_elem<D>(rec, fmt, t, e);
   if (fmt == TSB200_KV_INT8)
     return (float)(int8_t)rec[e * 16 + t] * reinterpret_cast<const float*>(rec + 16 * D)[t];

@@ -12,6 +12,7 @@
 //   nvfp4 : per 16 elements sb = e4m3_satfinite(amax/6), code = e2m1_satfinite(x/decode(sb))
 #include <type_traits>
 #include "common.cuh"
+#include "kv_page.cuh"
 
 namespace tsb {
 
@@ -833,9 +834,14 @@ int launch_append(const tsb200_kv_desc& kv, void* q, int64_t qs, int qheads, con
   return TSB200_OK;
 }
 
+// Pages that carry their own scale (kv_append_page.cu).
+template <typename T, int D>
+int launch_append_page(const tsb200_kv_desc& kv, void* q, int64_t qs, int qheads, const void* k, const void* v, int64_t ks, int64_t vs, int64_t B,
+                       int64_t Tn, const int32_t* new_lens, const float* rc, const float* rs, int64_t rr, cudaStream_t s);
+
 int validate_kv(const tsb200_kv_desc* kv, bool need_table) {
   if (!kv) return TSB200_ERR_ARG;
-  if (kv->format < 0 || kv->format > TSB200_KV_BF16) return TSB200_ERR_UNSUPPORTED;
+  if (kv->format < 0 || kv->format > TSB200_KV_FP8_PAGE) return TSB200_ERR_UNSUPPORTED;
   if (kv->head_dim != 64 && kv->head_dim != 128) return TSB200_ERR_UNSUPPORTED;
   if (kv->hkv <= 0 || kv->num_pages < 0 || kv->bt_stride < 0) return TSB200_ERR_ARG;
   if (!kv->k_pool || !kv->v_pool || !aligned(kv->k_pool, 16) || !aligned(kv->v_pool, 16)) return TSB200_ERR_ARG;
@@ -858,6 +864,7 @@ size_t tsb200_kv_record_bytes(int format, int head_dim) {
     case TSB200_KV_NVFP4: return (size_t)16 * head_dim / 2 + (size_t)head_dim;
     case TSB200_KV_F32: return (size_t)16 * head_dim * 4;
     case TSB200_KV_BF16: return (size_t)16 * head_dim * 2;
+    case TSB200_KV_FP8_PAGE: return (size_t)page_record_bytes(head_dim);
     default: return 0;
   }
 }
@@ -930,6 +937,11 @@ int tsb200_rope_append(const tsb200_kv_desc* kv, void* q, int q_heads, int64_t q
   const int64_t qs = q_token_stride ? q_token_stride : (int64_t)q_heads * kv->head_dim;
   if (ks < dense || vs < dense || (q && qs < (int64_t)q_heads * kv->head_dim)) return TSB200_ERR_ARG;
   cudaStream_t s = as_stream(stream);
+  if (kv->format == TSB200_KV_FP8_PAGE) {
+    auto go = dtype == TSB200_F32 ? (kv->head_dim == 64 ? launch_append_page<float, 64> : launch_append_page<float, 128>)
+                                  : (kv->head_dim == 64 ? launch_append_page<__nv_bfloat16, 64> : launch_append_page<__nv_bfloat16, 128>);
+    return go(*kv, q, qs, q_heads, k, v, ks, vs, B, T, new_lens, rope_cos, rope_sin, rope_rows, s);
+  }
   if (dtype == TSB200_F32)
     return kv->head_dim == 64 ? launch_append<float, 64>(*kv, q, qs, q_heads, k, v, ks, vs, B, T, new_lens, rope_cos, rope_sin, rope_rows, s)
                               : launch_append<float, 128>(*kv, q, qs, q_heads, k, v, ks, vs, B, T, new_lens, rope_cos, rope_sin, rope_rows, s);

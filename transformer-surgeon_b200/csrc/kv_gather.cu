@@ -6,6 +6,7 @@
 // block per (sequence, token), one thread per (kv head, element) pair group.  Positions at or
 // beyond seq_lens[b] are written as zeros.  HBM-bound and used once per prompt.
 #include "decode_attn_common.cuh"
+#include "kv_page.cuh"
 
 namespace tsb {
 namespace {
@@ -18,6 +19,7 @@ __global__ void kv_gather_kernel(tsb200_kv_desc kv, T* __restrict__ k_out, T* __
   const int len = kv.seq_lens[b];
   const int rec_bytes = kv.format == TSB200_KV_INT8 ? 16 * D + 64
                         : kv.format == TSB200_KV_FP8 ? 16 * D
+                        : kv.format == TSB200_KV_FP8_PAGE ? page_record_bytes(D)
                         : kv.format == TSB200_KV_NVFP4 ? 9 * D
                         : kv.format == TSB200_KV_F32 ? 64 * D : 32 * D;
   const bool valid = t < len;

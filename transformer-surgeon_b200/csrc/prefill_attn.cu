@@ -24,6 +24,7 @@
 // Every mbarrier wait is bounded; on expiry the CTA records a code in the status word, frees its TMEM and returns.
 #include "tc_common.cuh"
 #include "decode_attn_common.cuh"
+#include "kv_page.cuh"
 
 namespace tsb {
 using namespace tc;
@@ -409,13 +410,13 @@ constexpr int kGatherTokens = 64;
 // Codes of eight consecutive elements of a K vector / eight consecutive tokens of a V element -> their values (fp8: unscaled).
 template <int D, int FMT>
 __device__ __forceinline__ void k_eight(const uint8_t* __restrict__ rec, int t, int e, float (&v)[8]) {
-  if constexpr (FMT == TSB200_KV_INT8 || FMT == TSB200_KV_FP8) {
+  if constexpr (FMT == TSB200_KV_INT8 || FMT == TSB200_KV_FP8 || FMT == TSB200_KV_FP8_PAGE) {
     const uint2 c = *reinterpret_cast<const uint2*>(rec + t * D + e);
-    const float s = FMT == TSB200_KV_INT8 ? reinterpret_cast<const float*>(rec + 16 * D)[t] : 1.0f;
+    const float s = FMT == TSB200_KV_FP8 ? 1.0f : reinterpret_cast<const float*>(rec + 16 * D)[FMT == TSB200_KV_INT8 ? t : 0];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const unsigned b = ((i < 4 ? c.x : c.y) >> (8 * (i & 3))) & 0xffu;
-      v[i] = FMT == TSB200_KV_INT8 ? (float)(int8_t)b * s : e4m3_byte_to_f32(b);
+      v[i] = FMT == TSB200_KV_INT8 ? (float)(int8_t)b * s : FMT == TSB200_KV_FP8 ? e4m3_byte_to_f32(b) : e4m3_byte_to_f32(b) * s;
     }
   } else if constexpr (FMT == TSB200_KV_NVFP4) {
     const unsigned c = *reinterpret_cast<const unsigned*>(rec + t * (D / 2) + (e >> 1));
@@ -429,12 +430,14 @@ __device__ __forceinline__ void k_eight(const uint8_t* __restrict__ rec, int t, 
 }
 template <int D, int FMT>
 __device__ __forceinline__ void v_eight(const uint8_t* __restrict__ rec, int t, int e, float (&v)[8]) {
-  if constexpr (FMT == TSB200_KV_INT8 || FMT == TSB200_KV_FP8) {
+  if constexpr (FMT == TSB200_KV_INT8 || FMT == TSB200_KV_FP8 || FMT == TSB200_KV_FP8_PAGE) {
     const uint2 c = *reinterpret_cast<const uint2*>(rec + e * 16 + t);
+    const float s = FMT == TSB200_KV_FP8_PAGE ? *reinterpret_cast<const float*>(rec + 16 * D) : 1.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const unsigned b = ((i < 4 ? c.x : c.y) >> (8 * (i & 3))) & 0xffu;
-      v[i] = FMT == TSB200_KV_INT8 ? (float)(int8_t)b * reinterpret_cast<const float*>(rec + 16 * D)[t + i] : e4m3_byte_to_f32(b);
+      v[i] = FMT == TSB200_KV_INT8 ? (float)(int8_t)b * reinterpret_cast<const float*>(rec + 16 * D)[t + i]
+             : FMT == TSB200_KV_FP8 ? e4m3_byte_to_f32(b) : e4m3_byte_to_f32(b) * s;
     }
   } else if constexpr (FMT == TSB200_KV_NVFP4) {
     const uint2 c = *reinterpret_cast<const uint2*>(rec + (e >> 1) * 16 + t);
@@ -462,7 +465,7 @@ template <int D, int FMT>
 __global__ void __launch_bounds__(256)
 kv_gather_heads_kernel(tsb200_kv_desc kv, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ vt_out, int64_t L, int64_t Lp) {
   constexpr int rec_bytes = FMT == TSB200_KV_INT8 ? 16 * D + 64 : FMT == TSB200_KV_FP8 ? 16 * D : FMT == TSB200_KV_NVFP4 ? 9 * D
-                            : FMT == TSB200_KV_F32 ? 64 * D : 32 * D;
+                            : FMT == TSB200_KV_F32 ? 64 * D : FMT == TSB200_KV_FP8_PAGE ? page_record_bytes(D) : 32 * D;
   constexpr int UNITS = kGatherTokens * D / 8, PER = UNITS / 256;
   pdl_launch_dependents();
   pdl_wait();
@@ -511,6 +514,7 @@ int launch_gather_heads(const tsb200_kv_desc& kv, void* k_out, void* vt_out, int
     case TSB200_KV_FP8: TSB_GO(TSB200_KV_FP8); break;
     case TSB200_KV_NVFP4: TSB_GO(TSB200_KV_NVFP4); break;
     case TSB200_KV_F32: TSB_GO(TSB200_KV_F32); break;
+    case TSB200_KV_FP8_PAGE: TSB_GO(TSB200_KV_FP8_PAGE); break;
     default: TSB_GO(TSB200_KV_BF16);
   }
 #undef TSB_GO

@@ -33,7 +33,7 @@ class DecoderConfig:
     rms_eps: float = 1e-6
     norm_variant: int = 0          # 0 = Hugging Face RMSNorm, 1 = blocks/norm.py RMSNorm
     dtype: torch.dtype = torch.bfloat16
-    kv_format: str = "fp8"         # int8 | fp8 | nvfp4 | fp32 | bf16
+    kv_format: str = "fp8"         # int8 | fp8 | nvfp4 | fp32 | bf16 | fp8_page
     max_positions: int = 4096
     tp_world: int = 1              # tensor-parallel group size (1 = none); num_heads / num_kv_heads are GLOBAL
     tp_rank: int = 0
@@ -143,6 +143,7 @@ class CompressedDecoder:
         # `next_tokens` is updated) instead of lm_head -> logits -> argmax.  Set before capture().
         self.greedy_head = False
         self.head_ws = None
+        self._beams = None                  # ops.BeamReorder of the caches, once beam_search() ran
 
     def enable_peer_allreduce(self):
         """Tensor parallel: sum the row-parallel partial outputs with the library's own kernel over NVLink
@@ -283,6 +284,8 @@ class CompressedDecoder:
 
     def reset(self):
         self.seq_lens.zero_()
+        if self._beams is not None:
+            self._beams.reset()
 
     def bind_caches(self, kv, block_table, seq_lens):
         """Run on caller-owned caches (the blocks-path contract: the caller owns the caches and threads them
@@ -297,6 +300,9 @@ class CompressedDecoder:
                 raise ValueError("cache format / geometry differs from the engine's")
             if x.block_table is not block_table or x.seq_lens is not seq_lens:
                 raise ValueError("all layers must share one block table and one seq_lens tensor")
+        if self._beams is not None:
+            self._beams.reset()                  # the caches given back start with pages of their own
+            self._beams = None
         self.kv, self.block_table, self.seq_lens = list(kv), block_table, seq_lens
         self.pages_per_seq = block_table.shape[1]
         self.max_seq_len = min(self.max_seq_len, self.pages_per_seq * ops.PAGE)
@@ -372,6 +378,44 @@ class CompressedDecoder:
         self.lm_head(self.xn, out=self.logits, ws=self.lin_ws)
         ops.argmax(self.logits, out=self.next_tokens)
         return self.logits
+
+    @torch.no_grad()
+    def beam_search(self, input_ids, max_new_tokens, num_beams, eos_token_id=None, pad_token_id=None):
+        """Beam search over input_ids [B, T] on an engine built for B * num_beams sequences: every step keeps the num_beams best continuations
+        of a sequence by their summed log probabilities, and the caches follow them (full pages are shared between beams).  With eos_token_id a
+        beam that ends stays as it is, padded with pad_token_id (default: eos_token_id).  Returns (sequences int64 [B, num_beams, T + max_new_tokens],
+        scores fp32 [B, num_beams]), best first.  The prompt goes through prefill()."""
+        ids = input_ids.to(self.device)
+        B, T = ids.shape
+        K = int(num_beams)
+        if K < 1 or B * K != self.B:
+            raise ValueError(f"engine was built for {self.B} sequences, beam search needs {B} x {K}")
+        if self.greedy_head:
+            raise ValueError("beam search needs the step's logits: set greedy_head = False before capture()")
+        if max_new_tokens < 1 or T + max_new_tokens - 1 > self.max_seq_len:
+            raise ValueError("prompt and new tokens do not fit the engine")
+        pad = eos_token_id if pad_token_id is None else pad_token_id
+        if self._beams is None:
+            self._beams = ops.BeamReorder(self.kv)
+        logits = self.prefill(ids.repeat_interleave(K, dim=0))
+        # all beams are one beam at first: the others have no continuations yet
+        scores = torch.full((B, K), float("-inf"), dtype=torch.float32, device=self.device)
+        scores[:, 0] = 0.0
+        finished = None if eos_token_id is None else torch.zeros((B, K), dtype=torch.bool, device=self.device)
+        ws = torch.empty(ops.beam_select_workspace_bytes(B, K, logits.shape[1], logits.dtype, K), dtype=torch.uint8, device=self.device)
+        new = torch.empty((B * K, max_new_tokens), dtype=torch.int64, device=self.device)
+        for i in range(max_new_tokens):
+            scores, parents, tokens = ops.beam_select(logits, scores, K, finished=finished, pad_token=pad or 0, ws=ws)
+            rows, tokens = parents.view(-1), tokens.view(-1)
+            new = new.index_select(0, rows)
+            new[:, i] = tokens
+            if finished is not None:
+                finished = finished.view(-1).index_select(0, rows).logical_or_(tokens == eos_token_id).view(B, K)
+            if i + 1 < max_new_tokens:
+                self._beams(rows, self.seq_lens)
+                logits = self.step(tokens)
+        self.check_status()
+        return torch.cat((ids[:, None].expand(B, K, T), new.view(B, K, max_new_tokens)), dim=2), scores
 
     @torch.no_grad()
     def generate(self, input_ids, max_new_tokens, batched_prefill=None):

@@ -18,8 +18,11 @@ Usage (generate() itself is untouched):
     cache = PagedQuantCache(model.config, batch, max_len, kv_format="int8")
     model.generate(ids, past_key_values=cache, do_sample=False, ...)
 
+Beam search: build the cache for batch * num_beams sequences; `reorder_cache` shares the beams' full pages through the block
+table and copies the open ones (`tsb200_kv_reorder`).
+
 Limits: every sequence of the batch has the same length and the mask is the plain causal one (a padded
-batch is refused when first met); no beam reordering, cropping or sliding windows.
+batch is refused when first met); no cropping or sliding windows.
 """
 import torch
 from transformers import AttentionInterface
@@ -80,6 +83,7 @@ class PagedCacheLayer(CacheLayerMixin):
         return self.max_len
 
     def reset(self):
+        torch.arange(self.block_table.numel(), out=self.block_table.view(-1))     # every sequence its own pages again
         self.seq_lens.zero_()
         self.cumulative_length = 0
         self.mask_checked = False
@@ -97,7 +101,14 @@ class PagedQuantCache(Cache):
         head_dim = getattr(text, "head_dim", None) or text.hidden_size // text.num_attention_heads
         device = torch.device(device)
         layers = [PagedCacheLayer(kv_format, batch, max_len, hkv, head_dim, device, i) for i in range(text.num_hidden_layers)]
+        for layer in layers[1:]:                # one block table: a reordering is the same for all layers
+            layer.block_table = layer.kv.block_table = layers[0].block_table
         super().__init__(layers=layers)
+        self._reorder = ops.BeamReorder([layer.kv for layer in layers])
+
+    def reorder_cache(self, beam_idx):
+        """Row r continues from row beam_idx[r] (beam search): all layers in one launch."""
+        self._reorder(beam_idx.to(device=self.layers[0].device, dtype=torch.int32).contiguous())
 
 
 def _check_plain_causal(layer, attention_mask, T, L):

@@ -8,12 +8,12 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import F32, BF16, KV_INT8, KV_FP8, KV_NVFP4, KV_F32, KV_BF16, LinearDesc, KVDesc, NormDesc, check
+from ._lib import F32, BF16, KV_INT8, KV_FP8, KV_NVFP4, KV_F32, KV_BF16, KV_FP8_PAGE, LinearDesc, KVDesc, NormDesc, check
 
 from ._lib import Tsb200Error  # noqa: F401  (re-exported)
 
 ATTN_STATUS_OFFSET = 16380      # byte offset of the status word inside an attention workspace (last int of the counter block)
-KV_FORMATS = {"int8": KV_INT8, "fp8": KV_FP8, "nvfp4": KV_NVFP4, "fp32": KV_F32, "bf16": KV_BF16}
+KV_FORMATS = {"int8": KV_INT8, "fp8": KV_FP8, "nvfp4": KV_NVFP4, "fp32": KV_F32, "bf16": KV_BF16, "fp8_page": KV_FP8_PAGE}
 PAGE = 16
 
 
@@ -436,15 +436,19 @@ class PagedKV:
 
     flags = 0          # _lib.KV_FRESH: see the header
 
-    def __init__(self, fmt, num_pages, hkv, head_dim, block_table, seq_lens, device, k_scale=None, v_scale=None):
+    def __init__(self, fmt, num_pages, hkv, head_dim, block_table, seq_lens, device, k_scale=None, v_scale=None, k_pool=None, v_pool=None):
+        """k_pool, v_pool: memory the caller has already (uint8 [num_pages, hkv, record bytes], of finite codes); allocated otherwise."""
         self.fmt = KV_FORMATS[fmt] if isinstance(fmt, str) else fmt
         self.hkv, self.head_dim, self.num_pages = hkv, head_dim, num_pages
         self.rec = kv_record_bytes(self.fmt, head_dim)
         if self.rec == 0:
             raise ValueError("unsupported KV format / head_dim")
         # zero-initialised once: stale slots must hold finite codes and scales
-        self.k_pool = torch.zeros((num_pages, hkv, self.rec), dtype=torch.uint8, device=device)
-        self.v_pool = torch.zeros((num_pages, hkv, self.rec), dtype=torch.uint8, device=device)
+        for pool, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
+            if pool is not None and (pool.dtype != torch.uint8 or tuple(_cuda(pool, name).shape) != (num_pages, hkv, self.rec)):
+                raise ValueError(f"{name} must be uint8 [num_pages, hkv, record bytes] = [{num_pages}, {hkv}, {self.rec}]")
+        self.k_pool = torch.zeros((num_pages, hkv, self.rec), dtype=torch.uint8, device=device) if k_pool is None else k_pool
+        self.v_pool = torch.zeros((num_pages, hkv, self.rec), dtype=torch.uint8, device=device) if v_pool is None else v_pool
         self.block_table = block_table     # int32 [B, pages_per_seq] (shared between layers)
         self.seq_lens = seq_lens           # int32 [B]               (shared between layers)
         B = block_table.shape[0]
@@ -508,6 +512,54 @@ class PagedKV:
         check(lib.tsb200_kv_append(C.byref(d), _p(k), _p(v), _dt(k), ks, vs, B, T, _p(new_lens),
                                    _p(cos), _p(sin), 0 if cos is None else cos.shape[0], _stream()),
               "tsb200_kv_append")
+
+
+class BeamReorder:
+    """Beam search's reordering of the caches of all layers: row r of the batch takes over the cached tokens of row parents[r].
+
+    kvs: one PagedKV per layer; they share one block table, whose rows name pages of their own when this is built.  Full pages are
+    shared through the block table, the open page is copied into the row's own: one launch, whatever the context.  Before a sequence is started
+    anew (seq_lens back to 0), `reset` gives every row its own pages again."""
+
+    def __init__(self, kvs):
+        self.kvs = list(kvs)
+        if not self.kvs:
+            raise ValueError("no caches to reorder")
+        a = self.kvs[0]
+        for x in self.kvs:
+            if x.fmt != a.fmt or x.hkv != a.hkv or x.head_dim != a.head_dim or x.num_pages != a.num_pages:
+                raise ValueError("all layers must have the same format, heads and number of pages")
+            if x.block_table is not a.block_table:
+                raise ValueError("all layers must share one block table")
+        self.block_table, self.seq_lens = a.block_table, a.seq_lens
+        _cuda(self.block_table, "block_table")
+        self.home = self.block_table.clone()
+        ids = self.home.flatten().sort().values
+        if bool((ids[1:] == ids[:-1]).any()):
+            raise ValueError("every row of the block table must have pages of its own")
+        dev = self.block_table.device
+        pools = [p for x in self.kvs for p in (x.k_pool, x.v_pool)]
+        scales = [p for x in self.kvs for p in (x.k_scale, x.v_scale) if p is not None]
+        for p in scales:
+            _cuda(p, "scale")
+        self._held = pools + scales                      # their addresses are what the next two hold
+        self._pools = torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64, device=dev)
+        self._scales = torch.tensor([p.data_ptr() for p in scales], dtype=torch.int64, device=dev) if scales else None
+        self._n = (len(pools), a.hkv * a.rec, a.num_pages, len(scales), a.hkv)
+
+    def __call__(self, parents, seq_lens=None):
+        """parents int32 [rows]; a row whose parent is itself, out of range or of another length keeps what it has.  seq_lens: tokens cached per
+        row, where that is not the first layer's tensor."""
+        rows, width = self.block_table.shape
+        lens = self.seq_lens if seq_lens is None else _cuda(seq_lens, "seq_lens")
+        if _cuda(parents, "parents").dtype != torch.int32 or parents.numel() != rows or lens.dtype != torch.int32 or lens.numel() != rows:
+            raise ValueError(f"parents and seq_lens must be int32 [{rows}]")
+        n_pools, page_bytes, pages, n_scales, hkv = self._n
+        check(_lib.load().tsb200_kv_reorder(_p(self._pools), n_pools, page_bytes, pages, _p(self._scales), n_scales, hkv, _p(self.block_table), width,
+                                            _p(lens), _p(parents), rows, _stream()), "tsb200_kv_reorder")
+
+    def reset(self):
+        self.block_table.copy_(self.home)
 
 
 def kv_gather(kv, L, dtype=torch.bfloat16, seq_lens=None):
@@ -606,6 +658,42 @@ def argmax(y, out=None):
         out = torch.empty(M, dtype=torch.int64, device=y.device)
     check(_lib.load().tsb200_argmax(y.data_ptr(), _dt(y), M, N, out.data_ptr(), _stream()), "tsb200_argmax")
     return out
+
+
+def beam_select(logits, scores, n=None, finished=None, pad_token=0, out=None, ws=None):
+    """The n best continuations of every sequence over its beams and the vocabulary (default: as many as it has beams).
+    logits [B * K, V] (or [B, K, V]; rows may be evenly strided), scores fp32 [B, K] of the beams: value = score + log_softmax(logits).  Returns
+    (values fp32, parents int32, tokens int64), [B, n] each, best first, ties to the lower beam and token; a parent is a row of the batch
+    (b * K + beam), as BeamReorder takes it.  finished: bool [B, K]; such a beam goes on as pad_token at its own score only.  A beam of score
+    -inf, or with a NaN or +inf among its logits, has no continuations; places without any are filled at -inf."""
+    B, K = scores.shape
+    if not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor (this library has no CPU path)")
+    if logits.dim() == 3:
+        logits = logits.flatten(0, 1)
+    V = logits.shape[1]
+    if logits.shape[0] != B * K or (V > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [B * K, V] with unit stride in the last dimension")
+    if scores.dtype != torch.float32:
+        raise TypeError("scores must be float32")
+    if finished is not None and (finished.dtype != torch.bool or finished.shape != scores.shape):
+        raise ValueError("finished must be bool, of scores' shape")
+    n = K if n is None else int(n)
+    dt = _dt(logits)
+    if out is None:
+        out = tuple(torch.empty((B, n), dtype=t, device=logits.device) for t in (torch.float32, torch.int32, torch.int64))
+    elif any(o.shape != (B, n) or o.dtype != t for o, t in zip(out, (torch.float32, torch.int32, torch.int64))):
+        raise ValueError("out must be float32, int32 and int64 tensors [B, n]")
+    if ws is None:
+        ws = workspace(logits.device, beam_select_workspace_bytes(B, K, V, logits.dtype, n), "beams")
+    stride = logits.stride(0) if B * K > 1 else V
+    check(_lib.load().tsb200_beam_select(_p(logits), dt, stride, B, K, V, _p(_cuda(scores, "scores")), 0 if finished is None else _p(_cuda(finished, "finished")),
+                                         int(pad_token), n, *(_p(_cuda(o, "out")) for o in out), _p(ws), ws.numel(), _stream()), "tsb200_beam_select")
+    return out
+
+
+def beam_select_workspace_bytes(B, K, V, dtype, n):
+    return int(_lib.load().tsb200_beam_select_workspace_bytes(B, K, V, F32 if dtype == torch.float32 else BF16, n))
 
 
 def rope_(x, cos, sin, pos0=None):
