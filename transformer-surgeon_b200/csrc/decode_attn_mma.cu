@@ -26,9 +26,8 @@
 
 namespace tsb {
 
-int choose_splits_page(int64_t B, int hkv, int64_t max_seq_len);
 int launch_attn_page(const tsb200_kv_desc& kv, const void* q, void* out, int dtype, int64_t qs, int64_t B, int H, float sm_scale, int64_t max_seq_len,
-                     float* ws, int* status, cudaStream_t st);
+                     float* ws, size_t ws_bytes, int* status, cudaStream_t st);
 template <typename T>
 int launch_attn_fp8(const tsb200_kv_desc& kv, const void* q, int64_t qs, int H, float sm_scale, int64_t max_seq_len, int S,
                     int64_t B, float* ws, void* out, int* status, cudaStream_t st);
@@ -490,7 +489,8 @@ using namespace tsb;
 // Bytes that serve a problem: counters + partials of choose_splits() splits, which no format's own split count exceeds
 // (tsb200_paged_decode_attn_workspace_bytes is the hkv-independent upper bound of this).
 static size_t attn_exact_workspace_bytes(const tsb200_kv_desc* kv, int64_t B, int H, int64_t max_seq_len) {
-  const int S = kv->format == TSB200_KV_FP8_PAGE ? choose_splits_page(B, kv->hkv, max_seq_len) : choose_splits(B, kv->hkv, max_seq_len);
+  if (kv->format == TSB200_KV_FP8_PAGE) return kAttnCounterBytes;      // splits as the scratch has room
+  const int S = choose_splits(B, kv->hkv, max_seq_len);
   return kAttnCounterBytes + (size_t)(B * H * S * (2 + kv->head_dim)) * sizeof(float);
 }
 
@@ -512,7 +512,7 @@ static int decode_attn_dispatch(const tsb200_kv_desc* kv, const void* q, void* o
   const bool room = n_ctr < (int64_t)(kAttnCounterBytes / sizeof(int));
   int* status = counters + kAttnStatusIndex;
   if (kv->format == TSB200_KV_FP8_PAGE)    // e4m3 pages with their own scales (decode_attn_page.cu)
-    return launch_attn_page(*kv, q, out, dtype, qs, B, H, sm_scale, max_seq_len, ws, status, s);
+    return launch_attn_page(*kv, q, out, dtype, qs, B, H, sm_scale, max_seq_len, ws, workspace_bytes - kAttnCounterBytes, status, s);
   if (kv->format > TSB200_KV_NVFP4)    // unquantized pages: fp32 math (decode_attn_dense.cu)
     return attn_dense(kv, q, out, dtype, qs, B, H, sm_scale, max_seq_len, ws, room ? counters : nullptr, s);
   if (kv->format == TSB200_KV_FP8 && D == 128 && H / kv->hkv <= 4) {

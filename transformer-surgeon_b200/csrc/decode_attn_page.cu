@@ -1,12 +1,18 @@
 // Split-K paged decode attention over e4m3 pages that carry their own scales (kv_page.cuh):
 //   out[h] = sum_t p_t V_t / sum_t p_t,  p_t = exp(sm_scale q_h . K_t),  K_t = 2^eK code, V_t = 2^eV code,  e per page.
-// The codes go to the tensor cores as they are (mma.sync m16n8k32 e4m3).  The scale of V joins the exponent:
-//   w_t = 2^(s_t + eV - M) <= 1,  numerator sum w_t code_t,  denominator sum w_t 2^-eV   (s_t in bits, M the running maximum of s_t + eV),
-// so that pages of any scales share one accumulator.
-// q and w are fed as sums of e4m3 terms, each 16 times finer than the one before (term t stands for code / 16^t): bf16 queries are two terms
-// exactly and weights keep 8 bits, fp32 takes four terms, 16 bits.  The 16 rows of an MMA are 8 heads x 2 terms or 4 heads x 4 terms, the tokens
-// of K and the elements of V its columns: a softmax row stays in the four lanes that feed the second product, and its weights are that
-// product's operand as they are.
+// The scale of V joins the exponent:
+//   w_t = 2^(s_t + eV - M + 8),  numerator sum w_t code_t,  denominator sum w_t 2^-eV   (s_t in bits; M is at most 6 below the largest s_t + eV so far),
+// so that pages of any scales share one accumulator and the maximum moves rarely.
+// Products run on warp-level f16 MMAs (m16n8k16), whose 16 rows are a page's tokens (elements of V) and whose 8 columns are query heads: 8 of bf16
+// (a query scaled by a power of two is an f16 number, weights keep 11 bits), 4 of fp32 in two f16 terms, code and rest * 2^11 (22 bits).  The
+// codes are widened to f16 pairs, one conversion for two; the e4m3 form of the MMA does the same in every instruction, to both operands: 850
+// instructions for two pages of 128, 300 here.  A word of four codes is a k-step of the first product and half a row of the second, with the
+// tokens of both in the order that makes the transposed weights (movmatrix) the second one's operand.
+//
+// Work: the pages of all (sequence, kv head) units in one row, cut into equal ranges, one per CTA of a grid that fills the device, and each of those
+// into equal ranges of its warps.  A warp streams its pages through a private ring (cp.async.bulk, K and V record) that does not drain between units; a unit that lies in one warp's range is done there, one that crosses warps is put together in shared memory at the CTA's
+// end, one that crosses CTAs by a second launch.  So lengths of any mixture keep every SM busy to the end: a CTA costs ~4 us beside its
+// pages (32 sequences x half to all of 2100 tokens, 32 / 8 heads: 256 CTAs of a unit each 29.4 us, 768 of a third 39.3).
 #include "tc_common.cuh"
 #include "decode_attn_common.cuh"
 #include "kv_page.cuh"
@@ -19,9 +25,11 @@ using tc::mbar_init;
 using tc::mbar_try_wait;
 using tc::smem_u32;
 
-constexpr int kWarps = 6;
-constexpr int kStages = 2;                  // page pairs in a warp's ring
+constexpr int kStages = 4;                  // pages in a warp's ring
+constexpr int kMaxRows = 1024;              // sequences of a launch
+constexpr unsigned kMinPages = 12;          // of a CTA's range
 constexpr unsigned kWaitLimit = 1u << 22;
+constexpr float kAhead = 6.f, kUp = 8.f;    // bits a score may be above M; bits weights are scaled up by (2^14 at most in f16)
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
@@ -29,11 +37,24 @@ __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, unsigned by
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned transposed(unsigned x) {     // of an 8 x 8 matrix of f16, a pair a lane
+  unsigned y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+// Four e4m3 codes -> f16 pairs (first, second) and (third, fourth).
+__device__ __forceinline__ void widen(unsigned w, unsigned& a, unsigned& b) {
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\ncvt.rn.f16x2.e4m3x2 %0, lo;\ncvt.rn.f16x2.e4m3x2 %1, hi;\n}\n" : "=r"(a), "=r"(b) : "r"(w));
 }
 __device__ __forceinline__ void ldmatrix4(unsigned (&r)[4], const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)) : "memory");
@@ -43,329 +64,557 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
-// Nearest e4m3 codes of four values, in one word; on return y holds 16 times what they leave over.
-__device__ __forceinline__ unsigned take_term(float (&y)[4]) {
-  const unsigned short lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-  const unsigned short hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
-  const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(lo, __NV_E4M3)));
-  const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(hi, __NV_E4M3)));
-  y[0] = (y[0] - a.x) * 16.f;
-  y[1] = (y[1] - a.y) * 16.f;
-  y[2] = (y[2] - b.x) * 16.f;
-  y[3] = (y[3] - b.y) * 16.f;
-  return (unsigned)lo | ((unsigned)hi << 16);
-}
-// The words of rows gid and gid + 8: terms 0 and 1, or (four terms) 0 and 1 in even rows, 2 and 3 in odd ones.
-template <int TERMS>
-__device__ __forceinline__ void terms_of_rows(float (&y)[4], bool odd, unsigned& row, unsigned& row8) {
-  row = take_term(y);
-  row8 = take_term(y);
-  if constexpr (TERMS == 4) {
-    const unsigned t2 = take_term(y), t3 = take_term(y);
-    if (odd) { row = t2; row8 = t3; }
-  }
-}
-// Sum over a head's terms of an accumulator's rows gid (hi) and gid + 8 (lo).
-template <int TERMS>
-__device__ __forceinline__ float add_terms(float hi, float lo, bool odd) {
-  float v = fmaf(lo, 1.f / 16.f, hi);
-  if constexpr (TERMS == 4) {
-    if (odd) v *= 1.f / 256.f;
-    v += __shfl_xor_sync(0xffffffffu, v, 4);
-  }
-  return v;
+// x = hi + lo * 2^-11 in f16.
+__device__ __forceinline__ unsigned two_terms(float x) {
+  const float hi = __half2float(__float2half_rn(x));
+  return pack_f16(hi, (x - hi) * 2048.f);
 }
 
-template <typename T, int D>
-struct Cfg {
-  static constexpr int TERMS = sizeof(T) == 2 ? 2 : 4, HEADS = 16 / TERMS;
-  static constexpr int REC = page_record_bytes(D), STAGE = 4 * REC;            // K_A, V_A, K_B, V_B
-  static constexpr int RING = kStages * STAGE;
-  static constexpr size_t SMEM = (size_t)kWarps * RING + kWarps * kStages * 8;
-  static_assert((size_t)kWarps * HEADS * (2 + D) * sizeof(float) <= (size_t)kWarps * RING, "the merge stays clear of the barriers");
+// Pages of sequence b.
+__device__ __forceinline__ int pages_of(const tsb200_kv_desc& kv, int64_t b, int64_t max_seq_len) {
+  const int64_t len = min((int64_t)kv.seq_lens[b], max_seq_len);
+  return len <= 0 ? 0 : (int)((len + 15) >> 4);
+}
+// Pages of a CTA's range.  per_min bounds the number of ranges that a unit can lie in.  (The launch's pages fit 31 bits.)
+__device__ __forceinline__ unsigned range_pages(unsigned total, unsigned ctas, unsigned per_min) { return max((total + ctas - 1) / ctas, per_min); }
+
+struct PageArgs {
+  int64_t qs, max_seq_len;
+  unsigned per_min;
+  int B, H, chunks, heads;        // heads: query heads of a unit (the last chunk of a kv head may have fewer)
+  int S;                          // partials of a (sequence, head) in the workspace; 0: ranges end where units end
+  float sm_scale;
+};
+
+// Position in the row of units: page p of n of unit (b, uh), `left` pages to go (this one among them).
+struct Cursor {
+  int b, uh, p, n, left;
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32, 2)
-decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, int64_t qs, int H, int chunks, float sm_scale, int64_t max_seq_len, int S,
-                        float* __restrict__ ws, T* __restrict__ out, int* __restrict__ status) {
+struct Cfg {
+  static constexpr int HEADS = sizeof(T) == 2 ? 8 : 4;
+  static constexpr int REC = page_record_bytes(D), STAGE = 2 * REC;            // K, V
+  static constexpr int RING = kStages * STAGE;
+  static size_t smem(int warps, int heads, int B) {
+    return (size_t)warps * (RING + heads * (2 + D) * sizeof(float) + kStages * 8) + (size_t)B * sizeof(int);
+  }
+  static_assert(HEADS * (2 + D) * (int)sizeof(float) <= RING, "a warp's last partial fits its ring");
+};
+
+template <typename T, int D, int NW>
+__global__ void __launch_bounds__(NW * 32, 2)
+decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, float* __restrict__ ws, T* __restrict__ out, int* __restrict__ status) {
   using C = Cfg<T, D>;
-  constexpr int TERMS = C::TERMS, HEADS = C::HEADS, REC = C::REC;
+  constexpr int HEADS = C::HEADS, REC = C::REC;
+  constexpr bool kTwo = HEADS == 4;                          // columns are two terms of a head
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int s_scan[NW];
+  // parts of a warp: of a unit that began before its range (0), of one that goes on behind it (1).  unit (or -1), its first (sequence, head), its
+  // heads, and the place of this CTA's part among the unit's
+  __shared__ int4 s_part[2][NW];
+  __shared__ unsigned s_ends;                                // warps in whose range the unit of part 0 ends
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int gid = lane >> 2, tid = lane & 3;
-  const bool odd = gid & 1;
-  const int ch = (int)(blockIdx.x % chunks), s = blockIdx.y;
-  const int64_t bh = blockIdx.x / chunks;
-  const int hk = (int)(bh % kv.hkv);
-  const int64_t b = bh / kv.hkv;
-  const int g = H / kv.hkv, g0 = ch * HEADS, gn = min(HEADS, g - g0);
+  const int column_head = kTwo ? gid >> 1 : gid;             // of the unit, as the columns of both products' operands
+  const int g = a.H / kv.hkv, HU = kv.hkv * a.chunks;
+  const int PART = a.heads * (2 + D);                        // floats of a partial: (m, l) per head, then the sums
 
   uint8_t* ring = smem + (size_t)w * C::RING;
-  unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + (size_t)kWarps * C::RING) + w * kStages;
+  float* parts = reinterpret_cast<float*>(smem + (size_t)NW * C::RING);           // [warps][PART]: of a unit that began before the warp's range
+  unsigned long long* bars = reinterpret_cast<unsigned long long*>(parts + NW * PART) + w * kStages;
+  int* cum = reinterpret_cast<int*>(reinterpret_cast<unsigned long long*>(parts + NW * PART) + NW * kStages);   // pages of the sequences up to and with b
   if (lane == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(&bars[i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    s_part[0][w].x = s_part[1][w].x = -1;
+    if (w == 0) s_ends = 0u;
   }
-  __syncwarp();
-  // Lanes 0 .. 3 copy one record each: K and V of a pair's first page, K and V of its second.
-  const int64_t rec_stride = (int64_t)kv.hkv * REC;
-  const uint8_t* pool = ((lane & 1) ? kv.v_pool : kv.k_pool) + (int64_t)hk * REC;
-  auto copy = [&](int stage, int records, int page) {
-    if (lane == 0) mbar_expect_tx(&bars[stage], (unsigned)(records * REC));
-    __syncwarp();
-    if (lane < records) {
-      const int64_t at = page < 0 ? 0 : (page >= kv.num_pages ? kv.num_pages - 1 : page);
-      bulk_g2s(ring + stage * C::STAGE + lane * REC, pool + at * rec_stride, REC, &bars[stage]);
+  // Lengths and block table are inputs that the launch directly before this one does not write (see the header): looked up ahead of the wait.
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += NW * 32) {
+    const int b = b0 + (int)threadIdx.x;
+    int v = b < a.B ? pages_of(kv, b, a.max_seq_len) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
     }
-  };
-  pdl_wait();
-  int len = kv.seq_lens[b];
-  len = len < 0 ? 0 : (len > max_seq_len ? (int)max_seq_len : len);
-  int pb, pe;
-  split_range(len, s, S, pb, pe);
-  // this warp's pages: pb + w, pb + w + kWarps, ...; consecutive two form a pair (one ring stage)
-  const int n_pages = pe - pb - w > 0 ? (pe - pb - w + kWarps - 1) / kWarps : 0;
-  const int n_pairs = (n_pages + 1) / 2;
-  const int32_t* table = kv.block_table + b * kv.bt_stride + pb + w;
-  auto look_up = [&](int pair) {
-    const int idx = 2 * pair + (lane >> 1);
-    return lane < 4 && idx < n_pages ? table[idx * kWarps] : 0;
-  };
-  auto issue = [&](int pair, int page) {
-    if (pair < n_pairs) copy(pair % kStages, 2 * pair + 1 < n_pages ? 4 : 2, page);
-  };
-  issue(0, look_up(0));
-  int next_page = look_up(1);
-
-  // ---- the query as the first product's operand: k-step 2 c + u of a lane covers elements 16 (tid + 4 c) + 8 u + [0, 8)
-  unsigned qf[D / 32][4];
-  float scf;                                                 // raw sum -> score in bits
+    if (lane == 31) s_scan[w] = v;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      if (i < w) v += s_scan[i];
+      total += s_scan[i];
+    }
+    if (b < a.B) cum[b] = before + v;
+    before += total;
+    __syncthreads();
+  }
+  const unsigned P = (unsigned)before * HU;
+  auto pages_at = [&](int b) { return cum[b] - (b ? cum[b - 1] : 0); };
+  auto unit_start = [&](int b, int uh) { return (unsigned)(b ? cum[b - 1] : 0) * HU + (unsigned)uh * pages_at(b); };
+  unsigned c0, c1, per = 0;
+  if (a.S) {
+    per = range_pages(P, gridDim.x, a.per_min);
+    c0 = min((uint64_t)P, (uint64_t)blockIdx.x * per);
+    c1 = min((uint64_t)P, (uint64_t)c0 + per);
+  } else {
+    const unsigned units = (unsigned)a.B * HU, each = (units + gridDim.x - 1) / gridDim.x;
+    const unsigned u0 = min(units, blockIdx.x * each), u1 = min(units, u0 + each);
+    c0 = u0 < units ? unit_start(u0 / HU, u0 % HU) : P;
+    c1 = u1 < units ? unit_start(u1 / HU, u1 % HU) : P;
+  }
+  Cursor at;
   {
-    const int head = TERMS == 2 ? gid : gid >> 1;
-    float x[D / 64][16];
-    const T* qp = q + b * qs + (int64_t)(hk * g + g0 + head) * D;
-    const bool vec = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(qs * (int64_t)sizeof(T))) & 15) == 0;
-    float amax = 0.f;
-    bool finite = true;
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-      const T* p = qp + 16 * (tid + 4 * c);
-      if (head < gn && vec) {
-        alignas(16) T e[16];
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[c][i] = to_f32<T>(e[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[c][i] = head < gn ? to_f32<T>(p[i]) : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        amax = fmaxf(amax, fabsf(x[c][i]));
-        finite = finite && fabsf(x[c][i]) < INFINITY;
+    const unsigned each = (c1 - c0) / NW, rest = (c1 - c0) % NW;
+    const unsigned x0 = c0 + w * each + min((unsigned)w, rest);
+    at.left = (int)(each + ((unsigned)w < rest));
+    at.b = at.uh = at.p = at.n = 0;
+    if (at.left > 0) {
+      // first sequence that ends behind x0: which 32, which of them
+      const int i0 = min(32 * lane + 31, a.B - 1);
+      int lo = 32 * (__ffs(__ballot_sync(0xffffffffu, (unsigned)cum[i0] * HU > x0)) - 1);
+      lo += __ffs(__ballot_sync(0xffffffffu, (unsigned)cum[min(lo + lane, a.B - 1)] * HU > x0)) - 1;
+      at.b = lo;
+      at.n = pages_at(lo);
+      const unsigned r = x0 - unit_start(lo, 0);
+      at.uh = (int)(r / (unsigned)at.n);
+      at.p = (int)(r % (unsigned)at.n);
+    }
+  }
+  auto advance = [&](Cursor& c) {
+    --c.left;
+    if (++c.p == c.n && c.left > 0) {
+      c.p = 0;
+      if (++c.uh == HU) {
+        c.uh = 0;
+        do ++c.b; while (cum[c.b] == cum[c.b - 1]);           // left > 0: there is one with pages
+        c.n = pages_at(c.b);
       }
     }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // the largest element to [128, 256): a power of two, so that no bit is lost
-    const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 126);
-    const float up = exp2_int(min(7 - e, 127));
-    scf = finite ? exp2_int(max(e - 7, -126)) * sm_scale * kLog2e : __int_as_float(0x7fc00000);
-    scf += __shfl_xor_sync(0xffffffffu, scf, 1) * 0.f;       // not a number in one lane: in the whole row
-    scf += __shfl_xor_sync(0xffffffffu, scf, 2) * 0.f;
+  };
+
+  // Lanes 0 and 1 copy K and V.  A page's number is looked up a round before its copies leave.
+  Cursor ahead = at;
+  int next_stage = 0;
+  const uint8_t* next_src = nullptr;
+  bool next = false;
+  const int64_t rec_stride = (int64_t)kv.hkv * REC;
+  auto look_up = [&]() {
+    next = ahead.left > 0;
+    if (next) {
+      if (lane < 2) {
+        const int page = kv.block_table[ahead.b * kv.bt_stride + ahead.p];
+        const int64_t pg = page < 0 ? 0 : (page >= kv.num_pages ? kv.num_pages - 1 : page);
+        const int hk = a.chunks == 1 ? ahead.uh : ahead.uh / a.chunks;
+        next_src = (lane ? kv.v_pool : kv.k_pool) + pg * rec_stride + (int64_t)hk * REC;
+      }
+      advance(ahead);
+    }
+  };
+  auto issue = [&]() {
+    if (next) {
+      if (lane == 0) mbar_expect_tx(&bars[next_stage], 2 * REC);
+      __syncwarp();
+      if (lane < 2) bulk_g2s(ring + next_stage * C::STAGE + lane * REC, next_src, REC, &bars[next_stage]);
+      next_stage = next_stage == kStages - 1 ? 0 : next_stage + 1;
+    }
+  };
+  // Elements of the column's query: 16 (tid + 4 c) + [0, 16)
+  T qraw[D / 64][16];
+  const bool qvec = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(a.qs * (int64_t)sizeof(T))) & 15) == 0;
+  auto load_query = [&](int b, int hk, int h0) {
+    const bool there = column_head < min(HEADS, g - h0);
+    const T* qp = q + b * a.qs + (int64_t)(hk * g + h0 + column_head) * D + 16 * tid;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int i = 0; i < (int)sizeof(T); ++i) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (there && qvec) {
+          v = *reinterpret_cast<const uint4*>(qp + 64 * c + i * (16 / (int)sizeof(T)));
+        } else if (there) {
+          alignas(16) T e[16 / sizeof(T)];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float y[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = x[c][8 * u + 4 * r + i] * up;
-          terms_of_rows<TERMS>(y, odd, qf[2 * c + u][2 * r], qf[2 * c + u][2 * r + 1]);
+          for (int j = 0; j < 16 / (int)sizeof(T); ++j) e[j] = qp[64 * c + i * (16 / (int)sizeof(T)) + j];
+          v = *reinterpret_cast<const uint4*>(e);
         }
+        *reinterpret_cast<uint4*>(&qraw[c][i * (16 / (int)sizeof(T))]) = v;
+      }
+  };
+  look_up();
+  pdl_wait();     // q and the newest token's pages come from the launches before
+  if (at.left > 0) load_query(at.b, at.uh / a.chunks, at.uh % a.chunks * HEADS);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    issue();
+    look_up();
   }
 
-  float o[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;
+  unsigned qf[D / 16][2];         // k-step 4 c + r: elements 16 (tid + 4 c) + 4 r + {0, 1}, {2, 3}
+  float scf[2];                   // raw sum -> score in bits, of the heads whose scores this lane holds: 2 tid and 2 tid + 1, or tid
+  float o[D / 16][4];
+  float m_run[2], l_run[2];
+  int p_first = 0, len = 0;
+  bool fresh = true, loaded = true, ok = true;
+  int stage = 0;
+  unsigned parity = 0;
 
-  bool ok = true;
-  for (int pair = 0; pair < n_pairs; ++pair) {
-    issue(pair + 1, next_page);
-    next_page = look_up(pair + 2);
+  while (at.left > 0) {
+    issue();
+    look_up();
+    const int hk = a.chunks == 1 ? at.uh : at.uh / a.chunks, h0 = a.chunks == 1 ? 0 : at.uh % a.chunks * HEADS;
+    if (fresh) {
+      if (!loaded) load_query(at.b, hk, h0);
+      fresh = loaded = false;
+      p_first = at.p;
+      len = (int)min((int64_t)kv.seq_lens[at.b], a.max_seq_len);
+      float amax = 0.f;
+      bool finite = true;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = fabsf(to_f32<T>(qraw[c][i]));
+          amax = fmaxf(amax, x);
+          finite = finite && x < INFINITY;
+        }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // the largest element to [128, 256), by a power of two
+      const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 126);
+      const float up = exp2_int(min(7 - e, 127));
+      float sc = finite ? exp2_int(max(e - 7, -126)) * a.sm_scale * kLog2e : __int_as_float(0x7fc00000);
+      sc += __shfl_xor_sync(0xffffffffu, sc, 1) * 0.f;       // not a number in one lane: in the whole column
+      sc += __shfl_xor_sync(0xffffffffu, sc, 2) * 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        scf[i] = __shfl_sync(0xffffffffu, sc, 4 * (2 * tid + (kTwo ? 0 : i)));
+        m_run[i] = -INFINITY;
+        l_run[i] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float x0 = to_f32<T>(qraw[c][4 * r + 2 * i]) * up, x1 = to_f32<T>(qraw[c][4 * r + 2 * i + 1]) * up;
+            if constexpr (kTwo) {
+              const unsigned t0 = two_terms(x0), t1 = two_terms(x1);
+              qf[4 * c + r][i] = __byte_perm(t0, t1, gid & 1 ? 0x7632 : 0x5410);
+            } else {
+              qf[4 * c + r][i] = pack_f16(x0, x1);
+            }
+          }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    }
     {
       unsigned spins = 0;
-      while (!mbar_try_wait(&bars[pair % kStages], (pair / kStages) & 1)) {
+      while (!mbar_try_wait(&bars[stage], parity)) {
         if (++spins > kWaitLimit) { ok = false; break; }
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
     }
-    const uint8_t* st = ring + (pair % kStages) * C::STAGE;
-    const bool two = 2 * pair + 1 < n_pages;
-    // ---- scores of tokens 4 tid .. + 3 of both pages, in bits, with the exponent of the page's V scale
-    float sv[2][4], iv[2] = {0.f, 0.f};
-    float mx = -INFINITY;
+    const uint8_t* sK = ring + stage * C::STAGE;
+    const uint8_t* sV = sK + REC;
+    // ---- scores: row r of the tile's upper half is token 4 (r / 2) + r % 2, of its lower half the one two behind
+    float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+    const int token = 4 * (gid >> 1) + (gid & 1);
+    {
+      const uint8_t* row = sK + token * D + 16 * tid;
 #pragma unroll
-    for (int X = 0; X < 2; ++X) {
+      for (int c = 0; c < D / 64; ++c) {
+        const uint4 ka = *reinterpret_cast<const uint4*>(row + 64 * c);
+        const uint4 kb = *reinterpret_cast<const uint4*>(row + 2 * D + 64 * c);
+        const unsigned wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sv[X][i] = -INFINITY;
-      if (X == 0 || two) {
-        const uint8_t* sK = st + X * 2 * REC;
-        const int nt = len - (pb + w + (2 * pair + X) * kWarps) * 16;       // tokens left from this page on
-        float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          // column n of n-tile j: token 4 (n / 2) + 2 j + n % 2, so that a lane's four columns are consecutive tokens
-          const uint8_t* row = sK + (4 * (gid >> 1) + 2 * j + (gid & 1)) * D;
-#pragma unroll
-          for (int h = 0; h < D / 64; ++h) {
-            const uint4 kk = *reinterpret_cast<const uint4*>(row + 16 * (tid + 4 * h));
-            mma_e4m3(c[j], qf[2 * h], kk.x, kk.y);
-            mma_e4m3(c[j], qf[2 * h + 1], kk.z, kk.w);
-          }
-        }
-        const float ks = scf * *reinterpret_cast<const float*>(sK + 16 * D);
-        const int ev = scale_exponent(*reinterpret_cast<const float*>(sK + REC + 16 * D));
-        iv[X] = exp2_int(-ev);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = add_terms<TERMS>(c[i >> 1][i & 1], c[i >> 1][2 + (i & 1)], odd);
-          if (4 * tid + i < nt) sv[X][i] = fmaf(v, ks, (float)ev);
-          mx = fmaxf(mx, sv[X][i]);
+        for (int r = 0; r < 4; ++r) {
+          unsigned a0, a1, a2, a3;
+          widen(wa[r], a0, a2);
+          widen(wb[r], a1, a3);
+          mma_f16(r & 1 ? c1 : c0, a0, a1, a2, a3, qf[4 * c + r][0], qf[4 * c + r][1]);
         }
       }
     }
-    // ---- online softmax: a row's maximum over its four lanes
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float mn = fmaxf(m_run, mx), ref = mn == -INFINITY ? 0.f : mn;
-    const float corr = ex2(m_run - ref);
-    const bool rescale = __any_sync(0xffffffffu, mn != m_run);
-    m_run = mn;
-    l_run *= corr;
-    unsigned pf[4];
+    const float ks = *reinterpret_cast<const float*>(sK + 16 * D);
+    const int ev = scale_exponent(*reinterpret_cast<const float*>(sV + 16 * D));
+    const int nt = len - at.p * 16;                           // tokens from this page on
+    const bool in0 = token < nt, in1 = token + 2 < nt;
+    // sv[half][head]: of the lane's two heads, or (two terms) the one
+    constexpr int N = kTwo ? 1 : 2;
+    float sv[2][N];
+    bool above = false;
 #pragma unroll
-    for (int X = 0; X < 2; ++X) {
-      float y[4], sum = 0.f;
+    for (int i = 0; i < N; ++i) {
+      const float f = scf[i] * ks;
+      const float lo = kTwo ? fmaf(c0[1] + c1[1], 1.f / 2048.f, c0[0] + c1[0]) : c0[i] + c1[i];
+      const float hi = kTwo ? fmaf(c0[3] + c1[3], 1.f / 2048.f, c0[2] + c1[2]) : c0[2 + i] + c1[2 + i];
+      sv[0][i] = in0 ? fmaf(lo, f, (float)ev) : -INFINITY;
+      sv[1][i] = in1 ? fmaf(hi, f, (float)ev) : -INFINITY;
+      above = above || fmaxf(sv[0][i], sv[1][i]) > m_run[i] + kAhead;
+    }
+    if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[i] = ex2(sv[X][i] - ref);
-        sum += y[i];
+      for (int i = 0; i < N; ++i) {
+        float mx = fmaxf(sv[0][i], sv[1][i]);
+#pragma unroll
+        for (int of = 4; of < 32; of <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, of));
+        mx = fmaxf(mx, m_run[i]);
+        const float corr = mx == -INFINITY ? 1.f : ex2(m_run[i] - mx);
+        m_run[i] = mx;
+        l_run[i] *= corr;
+        // accumulators of this lane: columns 2 tid and 2 tid + 1 (two terms: both of head tid)
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          o[j][i] *= corr;
+          o[j][2 + i] *= corr;
+          if (kTwo) { o[j][1] *= corr; o[j][3] *= corr; }
+        }
       }
-      l_run = fmaf(sum, iv[X], l_run);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] *= 256.f;
-      terms_of_rows<TERMS>(y, odd, pf[2 * X], pf[2 * X + 1]);
     }
-    // ---- O += w V: k-slots 4 tid .. + 3 are tokens 4 tid .. + 3 of the first page, the upper sixteen those of the second
-    if (rescale) {
+    const float iv = exp2_int(-ev);
+    float w0[N], w1[N];
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) { o[i][0] *= corr; o[i][1] *= corr; o[i][2] *= corr; o[i][3] *= corr; }
+    for (int i = 0; i < N; ++i) {
+      const float ref = (m_run[i] == -INFINITY ? 0.f : m_run[i]) - kUp;
+      w0[i] = ex2(sv[0][i] - ref);
+      w1[i] = ex2(sv[1][i] - ref);
+      l_run[i] = fmaf(w0[i] + w1[i], iv, l_run[i]);
     }
-    const uint8_t* sV = st + REC + lane * 16;
+    const unsigned b0 = transposed(kTwo ? two_terms(w0[0]) : pack_f16(w0[0], w0[N - 1]));
+    const unsigned b1 = transposed(kTwo ? two_terms(w1[0]) : pack_f16(w1[0], w1[N - 1]));
+    // ---- sums over the page's tokens: k-slots 2 tid, 2 tid + 1, 2 tid + 8, 2 tid + 9 are tokens 4 tid .. + 3
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
-      unsigned va[4], vb[4] = {0u, 0u, 0u, 0u};
-      ldmatrix4(va, sV + i * 512);
-      if (two) ldmatrix4(vb, sV + 2 * REC + i * 512);
+      unsigned va[4];
+      ldmatrix4(va, sV + lane * 16 + i * 512);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mma_e4m3(o[4 * i + j], pf, va[j], vb[j]);
+      for (int j = 0; j < 2; ++j) {
+        unsigned a0, a1, a2, a3;
+        widen(va[2 * j], a0, a2);
+        widen(va[2 * j + 1], a1, a3);
+        mma_f16(o[2 * i + j], a0, a1, a2, a3, b0, b1);
+      }
     }
     __syncwarp();     // all lanes are done with this stage before it is refilled
+    if (++stage == kStages) { stage = 0; parity ^= 1; }
+    // ---- the unit's last page in this range
+    if (at.left == 1 || at.p + 1 == at.n) {
+      fresh = true;
+      const bool begins = p_first == 0, ends = at.p + 1 == at.n;
+      float* part = begins ? reinterpret_cast<float*>(ring) : parts + w * PART;   // a unit that goes on is the range's last: its ring is empty
+      const int gn = min(HEADS, g - h0), oh = at.b * a.H + hk * g + h0;
+      if (!(begins && ends) && lane == 0) {
+        s_part[begins][w] = make_int4(at.b * HU + at.uh, oh, gn, a.S ? (int)(blockIdx.x - unit_start(at.b, at.uh) / per) : 0);
+        if (ends) atomicOr(&s_ends, 1u << w);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int of = 4; of < 32; of <<= 1) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], of);
+      }
+      T* dst = out + (int64_t)oh * D;
+      // accumulators of head tid (two terms), or of heads 2 tid and 2 tid + 1; rows are elements 16 j + gid and + 8
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int h = kTwo ? tid : 2 * tid + i;
+        if (h >= gn) continue;
+        const float inv = 1.f / l_run[i];
+        if (!(begins && ends) && gid == 0) *reinterpret_cast<float2*>(part + 2 * h) = make_float2(m_run[i], l_run[i]);
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          const float x0 = kTwo ? fmaf(o[j][1], 1.f / 2048.f, o[j][0]) : o[j][i], x1 = kTwo ? fmaf(o[j][3], 1.f / 2048.f, o[j][2]) : o[j][2 + i];
+          if (begins && ends) {
+            dst[h * D + 16 * j + gid] = from_f32<T>(x0 * inv);
+            dst[h * D + 16 * j + 8 + gid] = from_f32<T>(x1 * inv);
+          } else {
+            part[2 * a.heads + h * D + 16 * j + gid] = x0;
+            part[2 * a.heads + h * D + 16 * j + 8 + gid] = x1;
+          }
+        }
+      }
+    }
+    advance(at);
   }
   if (!ok) {
     // a wait ran out: give the copies in flight a bounded time to land before shared memory is reused, and record it
     if (lane == 0 && status) atomicMax(status, 8);
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
   }
+  __syncthreads();
 
-  // ---- the warps' results meet in shared memory
-  l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-  l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-  __syncthreads();
-  float* sm_m = reinterpret_cast<float*>(smem);              // [warps][HEADS]
-  float* sm_l = sm_m + kWarps * HEADS;
-  float* sm_acc = sm_l + kWarps * HEADS;                     // [warps][HEADS][D]
-  const int head = TERMS == 2 ? gid : gid >> 1;
-  if (tid == 0 && (TERMS == 2 || !odd)) {
-    sm_m[w * HEADS + head] = m_run;
-    sm_l[w * HEADS + head] = l_run;
-  }
+  // ---- units that cross warps.  A chain starts with a part of the second kind, or with the CTA's first part if that is of the first kind.
+  const int unit0 = lane < NW ? s_part[0][lane].x : -1, unit1 = lane < NW ? s_part[1][lane].x : -1;
+  const unsigned with0 = __ballot_sync(0xffffffffu, unit0 >= 0), with1 = __ballot_sync(0xffffffffu, unit1 >= 0), ending = s_ends;
+  const int lead = with0 && !(with1 & ((with0 & -with0) - 1u)) ? __ffs(with0) - 1 : -1;
+  int task = 0;
+#pragma unroll 1
+  for (unsigned starts = with1 << 1 | (lead >= 0); starts; starts &= starts - 1) {
+    const int f = __ffs(starts) - 2;                         // -1: the lead
+    const int fw = f < 0 ? lead : f;
+    const int4 info = s_part[f >= 0][fw];
+    unsigned members = f < 0 && (ending >> fw & 1) ? 0u : __ballot_sync(0xffffffffu, unit0 == info.x && lane > fw);
+    const unsigned last = members & ending;                  // the unit's last part
+    if (last) members &= (last << 1) - 1u;
+    const bool done = f >= 0 && last;
+    const float* first = f < 0 ? parts + fw * PART : reinterpret_cast<const float*>(smem + (size_t)fw * C::RING);
+#pragma unroll 1
+    for (int h = 0; h < info.z; ++h) {
+      if (task++ % NW != w) continue;
+      // lane i: the part of warp i, lane NW: the first
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (lane == NW || (members >> lane & 1)) ml = *reinterpret_cast<const float2*>((lane == NW ? first : parts + lane * PART) + 2 * h);
+      const float mm = warp_max(ml.x);
+      const float c = ml.x == -INFINITY ? 0.f : ex2(ml.x - mm);
+      const float ll = warp_sum(ml.y * c);
+      float acc[D / 32];
+      const float cf = __shfl_sync(0xffffffffu, c, NW);
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) {
-    const float a0 = add_terms<TERMS>(o[i][0], o[i][2], odd), a1 = add_terms<TERMS>(o[i][1], o[i][3], odd);
-    if (TERMS == 2 || !odd) *reinterpret_cast<float2*>(sm_acc + (size_t)(w * HEADS + head) * D + 8 * i + 2 * tid) = make_float2(a0, a1);
-  }
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < gn * D; idx += blockDim.x) {
-    const int i = idx / D, e = idx % D;
-    float mm = -INFINITY;
+      for (int i = 0; i < D / 32; ++i) acc[i] = first[2 * a.heads + h * D + lane + 32 * i] * cf;
 #pragma unroll
-    for (int ww = 0; ww < kWarps; ++ww) mm = fmaxf(mm, sm_m[ww * HEADS + i]);
-    float ll = 0.f, acc = 0.f;
+      for (int j = 1; j < NW; ++j) {
+        const float cj = __shfl_sync(0xffffffffu, c, j);
+        if (members >> j & 1) {
 #pragma unroll
-    for (int ww = 0; ww < kWarps; ++ww) {
-      const float mw = sm_m[ww * HEADS + i];
-      const float c = mw == -INFINITY ? 0.f : exp2f(mw - mm);
-      ll = fmaf(sm_l[ww * HEADS + i], c, ll);
-      acc = fmaf(sm_acc[(size_t)(ww * HEADS + i) * D + e], c, acc);
+          for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(parts[j * PART + 2 * a.heads + h * D + lane + 32 * i], cj, acc[i]);
+        }
+      }
+      const int64_t oh = info.y + h;
+      if (done) {
+        const float inv = 1.f / ll;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) out[oh * D + lane + 32 * i] = from_f32<T>(acc[i] * inv);
+      } else {
+        float* p = ws + (oh * a.S + info.w) * (2 + D);
+        if (lane == 0) *reinterpret_cast<float2*>(p) = make_float2(mm, ll);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) p[2 + lane + 32 * i] = acc[i];
+      }
     }
-    acc *= 1.f / 256.f;
-    const int64_t oh = b * H + hk * g + g0 + i;
-    if (S == 1) {
-      out[oh * D + e] = from_f32<T>(len > 0 ? acc / ll : 0.f);
-    } else {
-      float* p = ws + (oh * S + s) * (2 + D);
-      if (e == 0) { p[0] = mm * 0.6931471805599453f; p[1] = ll; }
-      p[2 + e] = acc;
-    }
   }
+  // ---- sequences without tokens
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (pages_at(b) == 0)
+      for (int i = threadIdx.x; i < a.H * D; i += NW * 32) out[(int64_t)b * a.H * D + i] = from_f32<T>(0.f);
 }
 
+// One CTA per (sequence, head), one thread per element: adds up the parts of a head whose unit crosses CTAs, in order.  Chained to the attention.
 template <typename T, int D>
-int launch(const tsb200_kv_desc& kv, const void* q, int64_t qs, int H, float sm_scale, int64_t max_seq_len, int S, int64_t B, float* ws, void* out,
-           int* status, cudaStream_t st) {
+__global__ void __launch_bounds__(D)
+decode_attn_page_join_kernel(tsb200_kv_desc kv, PageArgs a, int ctas, const float* __restrict__ ws, T* __restrict__ out) {
+  __shared__ int s_sum[2][D / 32];
+  pdl_launch_dependents();
+  const int t = threadIdx.x;
+  const int64_t oh = blockIdx.x;
+  const int b = (int)(oh / a.H), h = (int)(oh % a.H), g = a.H / kv.hkv;
+  int before = 0, all = 0;
+  for (int i = t; i < a.B; i += D) {
+    const int n = pages_of(kv, i, a.max_seq_len);
+    all += n;
+    before += i < b ? n : 0;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  all = __reduce_add_sync(0xffffffffu, all);
+  if ((t & 31) == 0) { s_sum[0][t >> 5] = before; s_sum[1][t >> 5] = all; }
+  __syncthreads();
+  before = all = 0;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) { before += s_sum[0][i]; all += s_sum[1][i]; }
+  const int HU = kv.hkv * a.chunks, uh = h / g * a.chunks + h % g / a.heads, n = pages_of(kv, b, a.max_seq_len);
+  const unsigned per = range_pages((unsigned)all * HU, ctas, a.per_min), start = (unsigned)before * HU + (unsigned)uh * n;
+  const int count = n == 0 ? 0 : (int)((start + n - 1) / per - start / per) + 1;
+  pdl_wait();
+  if (count < 2) return;
+  const float* p = ws + oh * a.S * (2 + D);
+  float mm = -INFINITY, ll = 0.f, acc = 0.f;
+  for (int i = 0; i < count; ++i) mm = fmaxf(mm, __ldcg(p + (int64_t)i * (2 + D)));
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + (int64_t)i * (2 + D)));
+    const float c = ml.x == -INFINITY ? 0.f : ex2(ml.x - mm);
+    ll = fmaf(ml.y, c, ll);
+    acc = fmaf(__ldcg(p + (int64_t)i * (2 + D) + 2 + t), c, acc);
+  }
+  out[oh * D + t] = from_f32<T>(acc / ll);
+}
+
+template <typename T, int D, int NW>
+int launch(tsb200_kv_desc kv, const T* q, PageArgs a, int64_t B, float* ws, T* out, int* status, cudaStream_t st) {
   using C = Cfg<T, D>;
   static bool configured[64] = {false};
   int dev = 0;
   TSB_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return TSB200_ERR_DEVICE;
   if (!configured[dev]) {
-    TSB_CUDA(cudaFuncSetAttribute(decode_attn_page_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+    TSB_CUDA(cudaFuncSetAttribute(decode_attn_page_kernel<T, D, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(NW, C::HEADS, kMaxRows)));
     configured[dev] = true;
   }
-  const int g = H / kv.hkv, chunks = (g + C::HEADS - 1) / C::HEADS;
-  if (B * kv.hkv * chunks > 0x7fffffffLL) return TSB200_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)(B * kv.hkv * chunks), (unsigned)S);
-  TSB_CUDA(launch_kernel_if(attn_overlaps(kv), decode_attn_page_kernel<T, D>, grid, dim3(kWarps * 32), C::SMEM, st, kv, (const T*)q, qs, H, chunks, sm_scale,
-                            max_seq_len, S, ws, (T*)out, status));
-  return S == 1 ? TSB200_OK : launch_reduce<T, D>(ws, B * H, S, out, st);
+  const int64_t units = (int64_t)kv.hkv * a.chunks, pages = units * ((a.max_seq_len + 15) / 16);      // of a sequence, at most
+  const int64_t rows = pages > 0 && 0x7fffffffLL / pages < kMaxRows ? 0x7fffffffLL / pages : kMaxRows;
+  if (rows < 1) return TSB200_ERR_UNSUPPORTED;
+  for (int64_t b = 0; b < B; b += rows) {
+    a.B = (int)(B - b < rows ? B - b : rows);
+    // two CTAs an SM, and no more than there can be ranges or units
+    const int64_t most = a.S ? (pages * a.B + a.per_min - 1) / a.per_min : units * a.B, ctas = most < 296 ? most : 296;
+    TSB_CUDA(launch_kernel_if(attn_overlaps(kv), decode_attn_page_kernel<T, D, NW>, dim3((unsigned)ctas), dim3(NW * 32), C::smem(NW, a.heads, a.B), st, kv, q, a, ws,
+                              out, status));
+    if (a.S)
+      TSB_CUDA(launch_kernel_if(true, decode_attn_page_join_kernel<T, D>, dim3((unsigned)(a.B * a.H)), dim3(D), 0, st, kv, a, (int)ctas, (const float*)ws, out));
+    kv.block_table += a.B * kv.bt_stride;
+    kv.seq_lens += a.B;
+    q += a.B * a.qs;
+    out += (int64_t)a.B * a.H * D;
+  }
+  return TSB200_OK;
+}
+
+template <typename T, int D>
+int launch_for(const tsb200_kv_desc& kv, const void* q, PageArgs a, int64_t B, float* ws, void* out, int* status, cudaStream_t st) {
+  constexpr int HEADS = Cfg<T, D>::HEADS;
+  const int g = a.H / kv.hkv;
+  a.chunks = (g + HEADS - 1) / HEADS;
+  a.heads = g < HEADS ? g : HEADS;
+  if ((int64_t)kMaxRows * a.H > 0x7fffffffLL || (int64_t)kv.hkv * a.chunks > 0x7fffffffLL / kMaxRows) return TSB200_ERR_UNSUPPORTED;
+  // two CTAs an SM: six warps each where their parts are small
+  return a.heads <= 4 ? launch<T, D, 6>(kv, (const T*)q, a, B, ws, (T*)out, status, st) : launch<T, D, 5>(kv, (const T*)q, a, B, ws, (T*)out, status, st);
 }
 
 }  // namespace
 
-int choose_splits_page(int64_t B, int hkv, int64_t max_seq_len) {
-  const int64_t base = B * hkv, pages = (max_seq_len + 15) / 16;
-  int64_t s = base > 0 ? (2 * 296 + base - 1) / base : 1;
-  const int64_t cap = pages / 24 > 0 ? pages / 24 : 1;
-  if (s > cap) s = cap;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// Whole units, if the most pages that a warp then gets are not many more than in equal ranges: the parts of cut units cost a launch and its
+// latency, about as long as a warp takes for nine pages.
+static bool whole_is_faster(int64_t units, int64_t pages) {
+  const int64_t whole = (units + 295) / 296 * ((pages + 5) / 6), cut = units * pages / (296 * 6);
+  return whole - cut <= 9;
 }
 
 int launch_attn_page(const tsb200_kv_desc& kv, const void* q, void* out, int dtype, int64_t qs, int64_t B, int H, float sm_scale, int64_t max_seq_len,
-                     float* ws, int* status, cudaStream_t st) {
-  const int S = choose_splits_page(B, kv.hkv, max_seq_len);
+                     float* ws, size_t ws_bytes, int* status, cudaStream_t st) {
+  PageArgs a = {};
+  a.qs = qs;
+  a.max_seq_len = max_seq_len;
+  a.H = H;
+  a.sm_scale = sm_scale;
+  // A unit lies in at most S ranges: no more than the workspace has room for.  Sequences of a few pages stay whole.
+  const int64_t pages = (max_seq_len + 15) / 16, room = (int64_t)(ws_bytes / ((size_t)(B * H) * (2 + kv.head_dim) * sizeof(float)));
+  int64_t S = pages / 4 < 64 ? pages / 4 : 64;
+  if (S > room) S = room;
+  a.S = S < 3 ? 0 : (int)S;
+  if (whole_is_faster(B * kv.hkv, pages)) a.S = 0;
+  if (a.S) {
+    a.per_min = (unsigned)((pages + a.S - 3) / (a.S - 2));
+    if (a.per_min < kMinPages) a.per_min = kMinPages;
+  }
   if (dtype == TSB200_F32)
-    return kv.head_dim == 64 ? launch<float, 64>(kv, q, qs, H, sm_scale, max_seq_len, S, B, ws, out, status, st)
-                             : launch<float, 128>(kv, q, qs, H, sm_scale, max_seq_len, S, B, ws, out, status, st);
-  return kv.head_dim == 64 ? launch<__nv_bfloat16, 64>(kv, q, qs, H, sm_scale, max_seq_len, S, B, ws, out, status, st)
-                           : launch<__nv_bfloat16, 128>(kv, q, qs, H, sm_scale, max_seq_len, S, B, ws, out, status, st);
+    return kv.head_dim == 64 ? launch_for<float, 64>(kv, q, a, B, ws, out, status, st) : launch_for<float, 128>(kv, q, a, B, ws, out, status, st);
+  return kv.head_dim == 64 ? launch_for<__nv_bfloat16, 64>(kv, q, a, B, ws, out, status, st)
+                           : launch_for<__nv_bfloat16, 128>(kv, q, a, B, ws, out, status, st);
 }
 
 }  // namespace tsb
