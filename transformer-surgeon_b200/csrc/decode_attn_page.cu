@@ -9,10 +9,11 @@
 // instructions for two pages of 128, 300 here.  A word of four codes is a k-step of the first product and half a row of the second, with the
 // tokens of both in the order that makes the transposed weights (movmatrix) the second one's operand.
 //
-// Work: the pages of all (sequence, kv head) units in one row, cut into equal ranges, one per CTA of a grid that fills the device, and each of those
-// into equal ranges of its warps.  A warp streams its pages through a private ring (cp.async.bulk, K and V record) that does not drain between units; a unit that lies in one warp's range is done there, one that crosses warps is put together in shared memory at the CTA's
-// end, one that crosses CTAs by a second launch.  So lengths of any mixture keep every SM busy to the end: a CTA costs ~4 us beside its
-// pages (32 sequences x half to all of 2100 tokens, 32 / 8 heads: 256 CTAs of a unit each 29.4 us, 768 of a third 39.3).
+// Work: the pages of all sequences in one row, cut into equal ranges, each for as many CTAs as there are kv heads, together as many as the device holds,
+// and each of those into equal ranges of its warps.  A warp streams its pages through a private ring (cp.async.bulk, K and V record) that does not
+// drain between sequences; a sequence that lies in one warp's range is done there, one that crosses warps is put together in shared memory
+// at the CTA's end, one that crosses ranges by a second launch.  So lengths of any mixture keep every SM busy to the end, and the heads of a page,
+// neighbours in memory, are read at about the same time (64 x 8192 tokens, 8 heads, pages in random order: 5.5 TB/s where they were not).
 #include "tc_common.cuh"
 #include "decode_attn_common.cuh"
 #include "kv_page.cuh"
@@ -25,9 +26,13 @@ using tc::mbar_init;
 using tc::mbar_try_wait;
 using tc::smem_u32;
 
-constexpr int kStages = 4;                  // pages in a warp's ring
+// Two CTAs of six warps with three pages each an SM (64 x 8192 tokens, 32 / 8 heads, 139 us; five warps and four pages 141, six and four, which
+// leaves the larger parts of more than four heads one CTA, 147, seven and three 146, eight and three 166).
+constexpr int NW = 6;
+constexpr int kStages = 3;                  // pages in a warp's ring
+constexpr int kSlots = 296;                 // CTAs that the device holds: two an SM
 constexpr int kMaxRows = 1024;              // sequences of a launch
-constexpr unsigned kMinPages = 12;          // of a CTA's range
+constexpr unsigned kMinPages = 6;           // of a range: one for every warp
 constexpr unsigned kWaitLimit = 1u << 22;
 constexpr float kAhead = 6.f, kUp = 8.f;    // bits a score may be above M; bits weights are scaled up by (2^14 at most in f16)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -75,20 +80,20 @@ __device__ __forceinline__ int pages_of(const tsb200_kv_desc& kv, int64_t b, int
   const int64_t len = min((int64_t)kv.seq_lens[b], max_seq_len);
   return len <= 0 ? 0 : (int)((len + 15) >> 4);
 }
-// Pages of a CTA's range.  per_min bounds the number of ranges that a unit can lie in.  (The launch's pages fit 31 bits.)
-__device__ __forceinline__ unsigned range_pages(unsigned total, unsigned ctas, unsigned per_min) { return max((total + ctas - 1) / ctas, per_min); }
+// Pages of a range.  per_min bounds the number of ranges that a sequence can lie in.  (The launch's pages fit 31 bits.)
+__device__ __forceinline__ unsigned range_pages(unsigned total, unsigned ranges, unsigned per_min) { return max((total + ranges - 1) / ranges, per_min); }
 
 struct PageArgs {
   int64_t qs, max_seq_len;
   unsigned per_min;
-  int B, H, chunks, heads;        // heads: query heads of a unit (the last chunk of a kv head may have fewer)
-  int S;                          // partials of a (sequence, head) in the workspace; 0: ranges end where units end
+  int B, H, chunks, heads;        // heads: query heads that a CTA takes of a kv head's, in so many chunks (the last may have fewer)
+  int S;                          // partials of a (sequence, head) in the workspace; 0: ranges end where sequences end
   float sm_scale;
 };
 
-// Position in the row of units: page p of n of unit (b, uh), `left` pages to go (this one among them).
+// Position in the row: page p of n of sequence b, `left` pages to go (this one among them).
 struct Cursor {
-  int b, uh, p, n, left;
+  int b, p, n, left;
 };
 
 template <typename T, int D>
@@ -96,13 +101,13 @@ struct Cfg {
   static constexpr int HEADS = sizeof(T) == 2 ? 8 : 4;
   static constexpr int REC = page_record_bytes(D), STAGE = 2 * REC;            // K, V
   static constexpr int RING = kStages * STAGE;
-  static size_t smem(int warps, int heads, int B) {
-    return (size_t)warps * (RING + heads * (2 + D) * sizeof(float) + kStages * 8) + (size_t)B * sizeof(int);
+  static size_t smem(int heads, int B) {
+    return (size_t)NW * (RING + heads * (2 + D) * sizeof(float) + kStages * 8) + (size_t)B * sizeof(int);
   }
   static_assert(HEADS * (2 + D) * (int)sizeof(float) <= RING, "a warp's last partial fits its ring");
 };
 
-template <typename T, int D, int NW>
+template <typename T, int D>
 __global__ void __launch_bounds__(NW * 32, 2)
 decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, float* __restrict__ ws, T* __restrict__ out, int* __restrict__ status) {
   using C = Cfg<T, D>;
@@ -110,19 +115,21 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
   constexpr bool kTwo = HEADS == 4;                          // columns are two terms of a head
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_scan[NW];
-  // parts of a warp: of a unit that began before its range (0), of one that goes on behind it (1).  unit (or -1), its first (sequence, head), its
-  // heads, and the place of this CTA's part among the unit's
-  __shared__ int4 s_part[2][NW];
-  __shared__ unsigned s_ends;                                // warps in whose range the unit of part 0 ends
+  // parts of a warp: of a sequence that began before its range (0), of one that goes on behind it (1): the sequence (or -1), and the place of
+  // this CTA's part among the sequence's
+  __shared__ int2 s_part[2][NW];
+  __shared__ unsigned s_ends;                                // warps in whose range the sequence of part 0 ends
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int gid = lane >> 2, tid = lane & 3;
-  const int column_head = kTwo ? gid >> 1 : gid;             // of the unit, as the columns of both products' operands
+  const int column_head = kTwo ? gid >> 1 : gid;             // of the CTA's, as the columns of both products' operands
   const int g = a.H / kv.hkv, HU = kv.hkv * a.chunks;
+  const int range = (int)blockIdx.x / HU, ranges = (int)gridDim.x / HU, uh = (int)blockIdx.x % HU;
+  const int hk = uh / a.chunks, h0 = uh % a.chunks * HEADS, gn = min(HEADS, g - h0);       // this CTA's heads: gn from hk g + h0 on
   const int PART = a.heads * (2 + D);                        // floats of a partial: (m, l) per head, then the sums
 
   uint8_t* ring = smem + (size_t)w * C::RING;
-  float* parts = reinterpret_cast<float*>(smem + (size_t)NW * C::RING);           // [warps][PART]: of a unit that began before the warp's range
+  float* parts = reinterpret_cast<float*>(smem + (size_t)NW * C::RING);           // [warps][PART]: of a sequence that began before the warp's range
   unsigned long long* bars = reinterpret_cast<unsigned long long*>(parts + NW * PART) + w * kStages;
   int* cum = reinterpret_cast<int*>(reinterpret_cast<unsigned long long*>(parts + NW * PART) + NW * kStages);   // pages of the sequences up to and with b
   if (lane == 0) {
@@ -153,47 +160,40 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
     before += total;
     __syncthreads();
   }
-  const unsigned P = (unsigned)before * HU;
-  auto pages_at = [&](int b) { return cum[b] - (b ? cum[b - 1] : 0); };
-  auto unit_start = [&](int b, int uh) { return (unsigned)(b ? cum[b - 1] : 0) * HU + (unsigned)uh * pages_at(b); };
+  const unsigned P = (unsigned)before;
+  auto start_of = [&](int b) { return (unsigned)(b ? cum[b - 1] : 0); };
   unsigned c0, c1, per = 0;
   if (a.S) {
-    per = range_pages(P, gridDim.x, a.per_min);
-    c0 = min((uint64_t)P, (uint64_t)blockIdx.x * per);
+    per = range_pages(P, ranges, a.per_min);
+    c0 = min((uint64_t)P, (uint64_t)range * per);
     c1 = min((uint64_t)P, (uint64_t)c0 + per);
   } else {
-    const unsigned units = (unsigned)a.B * HU, each = (units + gridDim.x - 1) / gridDim.x;
-    const unsigned u0 = min(units, blockIdx.x * each), u1 = min(units, u0 + each);
-    c0 = u0 < units ? unit_start(u0 / HU, u0 % HU) : P;
-    c1 = u1 < units ? unit_start(u1 / HU, u1 % HU) : P;
+    const int each = (a.B + ranges - 1) / ranges, b0 = range * each, b1 = b0 + each;
+    c0 = b0 < a.B ? start_of(b0) : P;
+    c1 = b1 < a.B ? start_of(b1) : P;
   }
   Cursor at;
   {
     const unsigned each = (c1 - c0) / NW, rest = (c1 - c0) % NW;
     const unsigned x0 = c0 + w * each + min((unsigned)w, rest);
     at.left = (int)(each + ((unsigned)w < rest));
-    at.b = at.uh = at.p = at.n = 0;
+    at.b = at.p = at.n = 0;
     if (at.left > 0) {
       // first sequence that ends behind x0: which 32, which of them
       const int i0 = min(32 * lane + 31, a.B - 1);
-      int lo = 32 * (__ffs(__ballot_sync(0xffffffffu, (unsigned)cum[i0] * HU > x0)) - 1);
-      lo += __ffs(__ballot_sync(0xffffffffu, (unsigned)cum[min(lo + lane, a.B - 1)] * HU > x0)) - 1;
+      int lo = 32 * (__ffs(__ballot_sync(0xffffffffu, (unsigned)cum[i0] > x0)) - 1);
+      lo += __ffs(__ballot_sync(0xffffffffu, (unsigned)cum[min(lo + lane, a.B - 1)] > x0)) - 1;
       at.b = lo;
-      at.n = pages_at(lo);
-      const unsigned r = x0 - unit_start(lo, 0);
-      at.uh = (int)(r / (unsigned)at.n);
-      at.p = (int)(r % (unsigned)at.n);
+      at.p = (int)(x0 - start_of(lo));
+      at.n = cum[lo] - (int)start_of(lo);
     }
   }
   auto advance = [&](Cursor& c) {
     --c.left;
     if (++c.p == c.n && c.left > 0) {
       c.p = 0;
-      if (++c.uh == HU) {
-        c.uh = 0;
-        do ++c.b; while (cum[c.b] == cum[c.b - 1]);           // left > 0: there is one with pages
-        c.n = pages_at(c.b);
-      }
+      do ++c.b; while (cum[c.b] == cum[c.b - 1]);             // left > 0: there is one with pages
+      c.n = cum[c.b] - cum[c.b - 1];
     }
   };
 
@@ -203,14 +203,14 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
   const uint8_t* next_src = nullptr;
   bool next = false;
   const int64_t rec_stride = (int64_t)kv.hkv * REC;
+  const uint8_t* pool = (lane ? kv.v_pool : kv.k_pool) + (int64_t)hk * REC;
   auto look_up = [&]() {
     next = ahead.left > 0;
     if (next) {
       if (lane < 2) {
         const int page = kv.block_table[ahead.b * kv.bt_stride + ahead.p];
         const int64_t pg = page < 0 ? 0 : (page >= kv.num_pages ? kv.num_pages - 1 : page);
-        const int hk = a.chunks == 1 ? ahead.uh : ahead.uh / a.chunks;
-        next_src = (lane ? kv.v_pool : kv.k_pool) + pg * rec_stride + (int64_t)hk * REC;
+        next_src = pool + pg * rec_stride;
       }
       advance(ahead);
     }
@@ -226,8 +226,8 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
   // Elements of the column's query: 16 (tid + 4 c) + [0, 16)
   T qraw[D / 64][16];
   const bool qvec = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(a.qs * (int64_t)sizeof(T))) & 15) == 0;
-  auto load_query = [&](int b, int hk, int h0) {
-    const bool there = column_head < min(HEADS, g - h0);
+  auto load_query = [&](int b) {
+    const bool there = column_head < gn;
     const T* qp = q + b * a.qs + (int64_t)(hk * g + h0 + column_head) * D + 16 * tid;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c)
@@ -247,7 +247,7 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
   };
   look_up();
   pdl_wait();     // q and the newest token's pages come from the launches before
-  if (at.left > 0) load_query(at.b, at.uh / a.chunks, at.uh % a.chunks * HEADS);
+  if (at.left > 0) load_query(at.b);
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
     issue();
@@ -266,9 +266,8 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
   while (at.left > 0) {
     issue();
     look_up();
-    const int hk = a.chunks == 1 ? at.uh : at.uh / a.chunks, h0 = a.chunks == 1 ? 0 : at.uh % a.chunks * HEADS;
     if (fresh) {
-      if (!loaded) load_query(at.b, hk, h0);
+      if (!loaded) load_query(at.b);
       fresh = loaded = false;
       p_first = at.p;
       len = (int)min((int64_t)kv.seq_lens[at.b], a.max_seq_len);
@@ -404,14 +403,13 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
     }
     __syncwarp();     // all lanes are done with this stage before it is refilled
     if (++stage == kStages) { stage = 0; parity ^= 1; }
-    // ---- the unit's last page in this range
+    // ---- the sequence's last page in this range
     if (at.left == 1 || at.p + 1 == at.n) {
       fresh = true;
       const bool begins = p_first == 0, ends = at.p + 1 == at.n;
-      float* part = begins ? reinterpret_cast<float*>(ring) : parts + w * PART;   // a unit that goes on is the range's last: its ring is empty
-      const int gn = min(HEADS, g - h0), oh = at.b * a.H + hk * g + h0;
+      float* part = begins ? reinterpret_cast<float*>(ring) : parts + w * PART;   // one that goes on is the range's last: its ring is empty
       if (!(begins && ends) && lane == 0) {
-        s_part[begins][w] = make_int4(at.b * HU + at.uh, oh, gn, a.S ? (int)(blockIdx.x - unit_start(at.b, at.uh) / per) : 0);
+        s_part[begins][w] = make_int2(at.b, a.S ? range - (int)(start_of(at.b) / per) : 0);
         if (ends) atomicOr(&s_ends, 1u << w);
       }
 #pragma unroll
@@ -419,7 +417,7 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
 #pragma unroll
         for (int of = 4; of < 32; of <<= 1) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], of);
       }
-      T* dst = out + (int64_t)oh * D;
+      T* dst = out + ((int64_t)at.b * a.H + hk * g + h0) * D;
       // accumulators of head tid (two terms), or of heads 2 tid and 2 tid + 1; rows are elements 16 j + gid and + 8
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -434,8 +432,8 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
             dst[h * D + 16 * j + gid] = from_f32<T>(x0 * inv);
             dst[h * D + 16 * j + 8 + gid] = from_f32<T>(x1 * inv);
           } else {
-            part[2 * a.heads + h * D + 16 * j + gid] = x0;
-            part[2 * a.heads + h * D + 16 * j + 8 + gid] = x1;
+            part[2 * a.heads + h * D + (16 * j + gid + 8 * tid) % D] = x0;        // turned by 8 elements a lane of the quad: no bank twice
+            part[2 * a.heads + h * D + (16 * j + 8 + gid + 8 * tid) % D] = x1;
           }
         }
       }
@@ -449,7 +447,7 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
   }
   __syncthreads();
 
-  // ---- units that cross warps.  A chain starts with a part of the second kind, or with the CTA's first part if that is of the first kind.
+  // ---- sequences that cross warps.  A chain starts with a part of the second kind, or with the CTA's first part if that is of the first kind.
   const int unit0 = lane < NW ? s_part[0][lane].x : -1, unit1 = lane < NW ? s_part[1][lane].x : -1;
   const unsigned with0 = __ballot_sync(0xffffffffu, unit0 >= 0), with1 = __ballot_sync(0xffffffffu, unit1 >= 0), ending = s_ends;
   const int lead = with0 && !(with1 & ((with0 & -with0) - 1u)) ? __ffs(with0) - 1 : -1;
@@ -458,14 +456,14 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
   for (unsigned starts = with1 << 1 | (lead >= 0); starts; starts &= starts - 1) {
     const int f = __ffs(starts) - 2;                         // -1: the lead
     const int fw = f < 0 ? lead : f;
-    const int4 info = s_part[f >= 0][fw];
+    const int2 info = s_part[f >= 0][fw];
     unsigned members = f < 0 && (ending >> fw & 1) ? 0u : __ballot_sync(0xffffffffu, unit0 == info.x && lane > fw);
-    const unsigned last = members & ending;                  // the unit's last part
+    const unsigned last = members & ending;                  // the sequence's last part
     if (last) members &= (last << 1) - 1u;
     const bool done = f >= 0 && last;
     const float* first = f < 0 ? parts + fw * PART : reinterpret_cast<const float*>(smem + (size_t)fw * C::RING);
 #pragma unroll 1
-    for (int h = 0; h < info.z; ++h) {
+    for (int h = 0; h < gn; ++h) {
       if (task++ % NW != w) continue;
       // lane i: the part of warp i, lane NW: the first
       float2 ml = make_float2(-INFINITY, 0.f);
@@ -473,25 +471,26 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
       const float mm = warp_max(ml.x);
       const float c = ml.x == -INFINITY ? 0.f : ex2(ml.x - mm);
       const float ll = warp_sum(ml.y * c);
+      const int turn = 8 * (kTwo ? h : h >> 1);
       float acc[D / 32];
       const float cf = __shfl_sync(0xffffffffu, c, NW);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] = first[2 * a.heads + h * D + lane + 32 * i] * cf;
+      for (int i = 0; i < D / 32; ++i) acc[i] = first[2 * a.heads + h * D + (lane + 32 * i + turn) % D] * cf;
 #pragma unroll
       for (int j = 1; j < NW; ++j) {
         const float cj = __shfl_sync(0xffffffffu, c, j);
         if (members >> j & 1) {
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(parts[j * PART + 2 * a.heads + h * D + lane + 32 * i], cj, acc[i]);
+          for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(parts[j * PART + 2 * a.heads + h * D + (lane + 32 * i + turn) % D], cj, acc[i]);
         }
       }
-      const int64_t oh = info.y + h;
+      const int64_t oh = (int64_t)info.x * a.H + hk * g + h0 + h;
       if (done) {
         const float inv = 1.f / ll;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) out[oh * D + lane + 32 * i] = from_f32<T>(acc[i] * inv);
       } else {
-        float* p = ws + (oh * a.S + info.w) * (2 + D);
+        float* p = ws + (oh * a.S + info.y) * (2 + D);
         if (lane == 0) *reinterpret_cast<float2*>(p) = make_float2(mm, ll);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) p[2 + lane + 32 * i] = acc[i];
@@ -500,19 +499,20 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
   }
   // ---- sequences without tokens
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-    if (pages_at(b) == 0)
+    if (cum[b] == (int)start_of(b))
       for (int i = threadIdx.x; i < a.H * D; i += NW * 32) out[(int64_t)b * a.H * D + i] = from_f32<T>(0.f);
 }
 
-// One CTA per (sequence, head), one thread per element: adds up the parts of a head whose unit crosses CTAs, in order.  Chained to the attention.
+// One CTA per (sequence, head), one thread per element: adds up the parts of a sequence that crosses ranges, in order.  Chained to the attention.
 template <typename T, int D>
 __global__ void __launch_bounds__(D)
-decode_attn_page_join_kernel(tsb200_kv_desc kv, PageArgs a, int ctas, const float* __restrict__ ws, T* __restrict__ out) {
+decode_attn_page_join_kernel(tsb200_kv_desc kv, PageArgs a, int ranges, const float* __restrict__ ws, T* __restrict__ out) {
   __shared__ int s_sum[2][D / 32];
+  __shared__ float s_c[64], s_l;
   pdl_launch_dependents();
   const int t = threadIdx.x;
   const int64_t oh = blockIdx.x;
-  const int b = (int)(oh / a.H), h = (int)(oh % a.H), g = a.H / kv.hkv;
+  const int b = (int)(oh / a.H);
   int before = 0, all = 0;
   for (int i = t; i < a.B; i += D) {
     const int n = pages_of(kv, i, a.max_seq_len);
@@ -526,25 +526,50 @@ decode_attn_page_join_kernel(tsb200_kv_desc kv, PageArgs a, int ctas, const floa
   before = all = 0;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) { before += s_sum[0][i]; all += s_sum[1][i]; }
-  const int HU = kv.hkv * a.chunks, uh = h / g * a.chunks + h % g / a.heads, n = pages_of(kv, b, a.max_seq_len);
-  const unsigned per = range_pages((unsigned)all * HU, ctas, a.per_min), start = (unsigned)before * HU + (unsigned)uh * n;
+  const int n = pages_of(kv, b, a.max_seq_len);
+  const unsigned per = range_pages((unsigned)all, ranges, a.per_min), start = (unsigned)before;
   const int count = n == 0 ? 0 : (int)((start + n - 1) / per - start / per) + 1;
   pdl_wait();
   if (count < 2) return;
+  // all parts' sums on their way while the coefficients are made
   const float* p = ws + oh * a.S * (2 + D);
-  float mm = -INFINITY, ll = 0.f, acc = 0.f;
-  for (int i = 0; i < count; ++i) mm = fmaxf(mm, __ldcg(p + (int64_t)i * (2 + D)));
-#pragma unroll 8
-  for (int i = 0; i < count; ++i) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + (int64_t)i * (2 + D)));
-    const float c = ml.x == -INFINITY ? 0.f : ex2(ml.x - mm);
-    ll = fmaf(ml.y, c, ll);
-    acc = fmaf(__ldcg(p + (int64_t)i * (2 + D) + 2 + t), c, acc);
+  constexpr int kFly = 16;
+  float v[kFly];
+#pragma unroll
+  for (int i = 0; i < kFly; ++i)
+    if (i < count) v[i] = __ldcg(p + (int64_t)i * (2 + D) + 2 + t);
+  if (t < 32) {
+    float2 ml[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      ml[i] = make_float2(-INFINITY, 0.f);
+      if (t + 32 * i < count) ml[i] = __ldcg(reinterpret_cast<const float2*>(p + (int64_t)(t + 32 * i) * (2 + D)));
+    }
+    const float mm = warp_max(fmaxf(ml[0].x, ml[1].x));
+    float ll = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float c = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - mm);
+      s_c[t + 32 * i] = c;
+      ll = fmaf(ml[i].y, c, ll);
+    }
+    ll = warp_sum(ll);
+    if (t == 0) s_l = ll;
   }
-  out[oh * D + t] = from_f32<T>(acc / ll);
+  __syncthreads();
+  float acc = 0.f;
+  for (int i0 = 0; i0 < count; i0 += kFly) {
+#pragma unroll
+    for (int i = 0; i < kFly; ++i)
+      if (i0 + i < count) acc = fmaf(v[i], s_c[i0 + i], acc);
+#pragma unroll
+    for (int i = 0; i < kFly; ++i)
+      if (i0 + kFly + i < count) v[i] = __ldcg(p + (int64_t)(i0 + kFly + i) * (2 + D) + 2 + t);
+  }
+  out[oh * D + t] = from_f32<T>(acc / s_l);
 }
 
-template <typename T, int D, int NW>
+template <typename T, int D>
 int launch(tsb200_kv_desc kv, const T* q, PageArgs a, int64_t B, float* ws, T* out, int* status, cudaStream_t st) {
   using C = Cfg<T, D>;
   static bool configured[64] = {false};
@@ -552,20 +577,23 @@ int launch(tsb200_kv_desc kv, const T* q, PageArgs a, int64_t B, float* ws, T* o
   TSB_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return TSB200_ERR_DEVICE;
   if (!configured[dev]) {
-    TSB_CUDA(cudaFuncSetAttribute(decode_attn_page_kernel<T, D, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(NW, C::HEADS, kMaxRows)));
+    TSB_CUDA(cudaFuncSetAttribute(decode_attn_page_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(C::HEADS, kMaxRows)));
     configured[dev] = true;
   }
-  const int64_t units = (int64_t)kv.hkv * a.chunks, pages = units * ((a.max_seq_len + 15) / 16);      // of a sequence, at most
+  const int64_t units = (int64_t)kv.hkv * a.chunks, pages = (a.max_seq_len + 15) / 16;
   const int64_t rows = pages > 0 && 0x7fffffffLL / pages < kMaxRows ? 0x7fffffffLL / pages : kMaxRows;
   if (rows < 1) return TSB200_ERR_UNSUPPORTED;
   for (int64_t b = 0; b < B; b += rows) {
     a.B = (int)(B - b < rows ? B - b : rows);
-    // two CTAs an SM, and no more than there can be ranges or units
-    const int64_t most = a.S ? (pages * a.B + a.per_min - 1) / a.per_min : units * a.B, ctas = most < 296 ? most : 296;
-    TSB_CUDA(launch_kernel_if(attn_overlaps(kv), decode_attn_page_kernel<T, D, NW>, dim3((unsigned)ctas), dim3(NW * 32), C::smem(NW, a.heads, a.B), st, kv, q, a, ws,
+    // two CTAs an SM, and no more than there can be ranges
+    const int64_t most = a.S ? (pages * a.B + a.per_min - 1) / a.per_min : a.B;
+    int64_t ranges = kSlots / units;
+    if (ranges > most) ranges = most;
+    if (ranges < 1) ranges = 1;
+    TSB_CUDA(launch_kernel_if(attn_overlaps(kv), decode_attn_page_kernel<T, D>, dim3((unsigned)(ranges * units)), dim3(NW * 32), C::smem(a.heads, a.B), st, kv, q, a, ws,
                               out, status));
     if (a.S)
-      TSB_CUDA(launch_kernel_if(true, decode_attn_page_join_kernel<T, D>, dim3((unsigned)(a.B * a.H)), dim3(D), 0, st, kv, a, (int)ctas, (const float*)ws, out));
+      TSB_CUDA(launch_kernel_if(true, decode_attn_page_join_kernel<T, D>, dim3((unsigned)(a.B * a.H)), dim3(D), 0, st, kv, a, (int)ranges, (const float*)ws, out));
     kv.block_table += a.B * kv.bt_stride;
     kv.seq_lens += a.B;
     q += a.B * a.qs;
@@ -580,18 +608,19 @@ int launch_for(const tsb200_kv_desc& kv, const void* q, PageArgs a, int64_t B, f
   const int g = a.H / kv.hkv;
   a.chunks = (g + HEADS - 1) / HEADS;
   a.heads = g < HEADS ? g : HEADS;
-  if ((int64_t)kMaxRows * a.H > 0x7fffffffLL || (int64_t)kv.hkv * a.chunks > 0x7fffffffLL / kMaxRows) return TSB200_ERR_UNSUPPORTED;
-  // two CTAs an SM: six warps each where their parts are small
-  return a.heads <= 4 ? launch<T, D, 6>(kv, (const T*)q, a, B, ws, (T*)out, status, st) : launch<T, D, 5>(kv, (const T*)q, a, B, ws, (T*)out, status, st);
+  if ((int64_t)kMaxRows * a.H > 0x7fffffffLL) return TSB200_ERR_UNSUPPORTED;
+  return launch<T, D>(kv, (const T*)q, a, B, ws, (T*)out, status, st);
 }
 
 }  // namespace
 
-// Whole units, if the most pages that a warp then gets are not many more than in equal ranges: the parts of cut units cost a launch and its
-// latency, about as long as a warp takes for nine pages.
-static bool whole_is_faster(int64_t units, int64_t pages) {
-  const int64_t whole = (units + 295) / 296 * ((pages + 5) / 6), cut = units * pages / (296 * 6);
-  return whole - cut <= 9;
+// Whole sequences, if the most pages that a warp then gets are not many more than in equal ranges: the parts of cut ones cost a launch, about as long as
+// a warp takes for five pages (whole / cut, us: 58 sequences x 575 tokens, 8 kv heads, 3 pages more: 19.1 / 21.3; 68 x 2076, 4 heads, 3: 30.7 / 32.6; 4 x 519,
+// 2 heads, 6: 8.1 / 7.4; 92 x 1660, 2 heads, 8: 22.0 / 18.7; 5 x 1491, 2 heads, 16: 17.7 / 8.5).
+static bool whole_is_faster(int64_t B, int64_t units, int64_t pages) {
+  const int64_t ranges = units < kSlots ? kSlots / units : 1;
+  const int64_t whole = (B + ranges - 1) / ranges * ((pages + NW - 1) / NW), cut = B * pages / (ranges * NW);
+  return whole - cut <= 5;
 }
 
 int launch_attn_page(const tsb200_kv_desc& kv, const void* q, void* out, int dtype, int64_t qs, int64_t B, int H, float sm_scale, int64_t max_seq_len,
@@ -601,12 +630,12 @@ int launch_attn_page(const tsb200_kv_desc& kv, const void* q, void* out, int dty
   a.max_seq_len = max_seq_len;
   a.H = H;
   a.sm_scale = sm_scale;
-  // A unit lies in at most S ranges: no more than the workspace has room for.  Sequences of a few pages stay whole.
+  // A sequence lies in at most S ranges: no more than the workspace has room for.  Sequences of a few pages stay whole.
   const int64_t pages = (max_seq_len + 15) / 16, room = (int64_t)(ws_bytes / ((size_t)(B * H) * (2 + kv.head_dim) * sizeof(float)));
   int64_t S = pages / 4 < 64 ? pages / 4 : 64;
   if (S > room) S = room;
   a.S = S < 3 ? 0 : (int)S;
-  if (whole_is_faster(B * kv.hkv, pages)) a.S = 0;
+  if (whole_is_faster(B, kv.hkv, pages)) a.S = 0;
   if (a.S) {
     a.per_min = (unsigned)((pages + a.S - 3) / (a.S - 2));
     if (a.per_min < kMinPages) a.per_min = kMinPages;
