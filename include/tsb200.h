@@ -309,7 +309,8 @@ int tsb200_kv_reorder(void* const* pools, int n_pools, int64_t page_bytes, int64
  * lowest k * V + t.  out_scores fp32, out_parents int32 (b * K + k: the row, as tsb200_kv_reorder takes it), out_tokens int64: [B, n].
  * finished (may be NULL): bytes [B, K]; a finished beam has one continuation, pad_token at its own score.  A beam whose score is -infinity or not a
  * number, or whose logits hold a NaN or +infinity, has none.  Where fewer than n values are above -infinity, the others are the lowest k * V + t left.
- * n <= 32, n <= K * V, K <= 256. */
+ * n <= 32, n <= K * V, K <= 256.  The first 16384 bytes of the workspace are counters: zero-fill them once before the first use; every completed call leaves them
+ * zero.  One workspace must not serve overlapping calls. */
 size_t tsb200_beam_select_workspace_bytes(int64_t B, int K, int64_t V, int dtype, int n);
 int tsb200_beam_select(const void* logits, int dtype, int64_t row_stride, int64_t B, int K, int64_t V, const float* scores,
                        const uint8_t* finished, int64_t pad_token, int n, float* out_scores, int32_t* out_parents, int64_t* out_tokens,

@@ -390,6 +390,12 @@ def test_select_hard_rows(cuda, name, kind):
     check_select(logits, scores, n)
 
 
+def test_select_more_sequences_than_counters(cuda):
+    g = torch.Generator().manual_seed(2)
+    logits, scores = torch.randn(2 * 4100, 40, generator=g).to(cuda), -torch.rand(4100, 2, generator=g).to(cuda)
+    check_select(logits, scores, 3)
+
+
 def test_select_dead_and_finished_beams(cuda):
     B, K, V, n = 6, 4, 5000, 8
     g = torch.Generator().manual_seed(2)
@@ -627,7 +633,7 @@ def test_select_and_reorder_captured(cuda):
         side.wait_stream(torch.cuda.current_stream())
         graph.replay()
         with torch.cuda.stream(side):
-            beside = ops.beam_select(other, torch.zeros(3, R, device=cuda), 2, ws=new_ws()[0].new_empty(1 << 20))
+            beside = ops.beam_select(other, torch.zeros(3, R, device=cuda), 2, ws=new_ws()[0].new_zeros(1 << 20))
         torch.cuda.synchronize()
         for a, b in zip(captured, want):
             assert torch.equal(a, b)

@@ -1,26 +1,31 @@
 // Beam search's selection: over the K * V continuations of a sequence,
 //   value[k, t] = score[k] + x[k, t] - logsumexp(x[k, :]),  the n largest, ties to the lowest k * V + t.
 //
-// One pass over the logits.  A CTA takes a stretch of one row: each thread sums exp(x - m) (m: its first maximum; fp32 over at most a few hundred
-// terms, 64 bits from there on, since candidates of different rows are told apart by less than 32 bits of a long sum hold) and puts elements that can
-// still be among the stretch's n largest aside.  What "can still be" means: the n-th largest of 128 group maxima of the stretch's first tile, a
-// value that n elements reach.  Elements put aside beyond the buffer raise that bound and the stretch is read once more; each such pass strictly
-// raises it, and the set that is left does not depend on the order of the atomics.
-// A second launch, chained to the first, adds up the rows' sums, turns the sorted lists into values in 64 bits and merges them.
-// Bound by the logits' bytes for many rows, by the two launches' latency for few.
+// One pass over the logits.  A CTA takes a stretch of one row, in vectors of 16 bytes: it sums 2^(x log2 e - R) (R: a whole number near the first
+// tile's maximum, so that sums are put together by exact shifts; fp32 over the few hundred terms of a thread, 64 bits from there on, since candidates of
+// different rows are told apart by less than 32 bits of a long sum hold) and notes vectors whose largest element can still be among the
+// stretch's n best.  What "can still be" means: the n-th largest of 64 group maxima of the first tile, a value that n elements reach.  At the end the n
+// best of the noted vectors hold the n best elements; those alone are looked at one by one.  More noted vectors than there is room for raise the
+// bound, and the stretch is read once more; each such pass strictly raises it, and what is left does not depend on the order of the atomics.
+// The last CTA of a sequence to be done adds up the rows' sums, turns the sorted lists into values in 64 bits and merges them (a second launch, even
+// chained to the first, took 2 us longer, and 4 on the host).
+// Bound by the logits' bytes for many rows (the exponential unit needs three quarters of that time), by the chain of steps behind them for few.
 #include "common.cuh"
 
 namespace tsb {
 namespace {
 
-constexpr int kThreads = 512, kVec = 2, kMaxBest = 32, kGroups = 128, kCap = 2048;
+constexpr int kThreads = 256, kVec = 4, kMaxBest = 32, kGroups = 64, kCap = 1024;
 constexpr int kMaxLists = 256, kMaxBeams = 256;
+constexpr int kCounters = 4096;         // sequences of a launch; their counters are the workspace's head
+constexpr int kMost = kMaxBest * (kMaxBest + 1);            // entries that can reach the merge's bound
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeast = -1e37f;       // a row of nothing above this (the type's lowest value as a mask) counts the elements equal to its maximum
 
 struct Part {           // of a row's stretch
-  double sum;           // sum of exp(x - m)
-  float m;
-  int pad;
+  double sum;           // sum of 2^(x log2 e - R)
+  float R;              // -infinity: the stretch has no element above kLeast,
+  float m;              // its maximum is this and `sum` the number of elements that have it
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -33,290 +38,431 @@ __device__ __forceinline__ bool before(float xa, int ia, float xb, int ib) { ret
 
 template <typename T>
 struct Row {
-  static constexpr int N = 16 / (int)sizeof(T);       // elements of a 16-byte vector
+  static constexpr int N = 16 / (int)sizeof(T);       // elements of a vector
   const T* base;                                      // 16-byte boundary at or below the row's first element
   int lead;                                           // elements between them
   int V;
   // elements v * N - lead .. of the row, -infinity where that is outside of it
-  __device__ __forceinline__ void load(int64_t v, float (&x)[N]) const {
-    const int64_t c0 = v * N - lead;
-    if (c0 >= 0 && c0 + N <= V) {
-      alignas(16) T e[N];
-      *reinterpret_cast<uint4*>(e) = __ldcs(reinterpret_cast<const uint4*>(base + v * N));
+  __device__ __forceinline__ uint4 load(int v) const {
+    const int c0 = v * N - lead;
+    if (c0 >= 0 && c0 <= V - N) return __ldcs(reinterpret_cast<const uint4*>(base) + v);
+    alignas(16) T e[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = to_f32<T>(e[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = c0 + i >= 0 && c0 + i < V ? to_f32<T>(base[v * N + i]) : -INFINITY;
-    }
+    for (int i = 0; i < N; ++i) e[i] = c0 + i >= 0 && c0 + i < V ? base[(int64_t)v * N + i] : from_f32<T>(-INFINITY);
+    return *reinterpret_cast<const uint4*>(e);
   }
 };
-
+// Largest element, NaN passed over (-infinity if there is none).
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-beam_rows_kernel(const T* __restrict__ logits, int64_t row_stride, int V, int splits, int64_t span, const float* __restrict__ scores,
-                 const uint8_t* __restrict__ finished, int n, Part* __restrict__ parts, float2* __restrict__ lists) {
-  constexpr int N = Row<T>::N;
-  __shared__ __align__(16) float s_group[kGroups];
-  __shared__ float s_x[kCap];
-  __shared__ int s_i[kCap];
-  __shared__ float s_bound;
-  __shared__ int s_group_i[kGroups], s_bound_i, s_count;
-  __shared__ double s_sum[kThreads / 32];
-  __shared__ float s_m[kThreads / 32];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int64_t row = blockIdx.x / splits;
-  const int split = (int)(blockIdx.x % splits), tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  // a row without a score or at its end has no candidates of its own
-  if (!(scores[row] > -INFINITY) || (finished && finished[row])) return;
-  Row<T> r;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(logits + row * row_stride);
-  r.base = reinterpret_cast<const T*>(at & ~(uintptr_t)15);
-  r.lead = (int)((at & 15) / sizeof(T));
-  r.V = V;
-  const int64_t vectors = (r.lead + (int64_t)V + N - 1) / N;
-  const int64_t v0 = split * span, v1 = min(vectors, v0 + span);
-  float m = -INFINITY, sum = 0.f;
-  if (tid == 0) { s_count = 0; s_bound = -INFINITY; }
-  float bound = -INFINITY;
-  auto put_aside = [&](float x, int64_t col) {
-    const int slot = atomicAdd(&s_count, 1);
-    if (slot < kCap) { s_x[slot] = x; s_i[slot] = (int)col; }
-  };
-  bool first = true;
-  for (int64_t t0 = v0; t0 < v1; t0 += kThreads * kVec) {
-    float x[kVec][N];
-#pragma unroll
-    for (int u = 0; u < kVec; ++u) {
-      const int64_t v = t0 + u * kThreads + tid;
-      if (v < v1) r.load(v, x[u]);
-      else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[u][i] = -INFINITY;
-      }
-    }
-    float top[kVec];
-#pragma unroll
-    for (int u = 0; u < kVec; ++u) {
-      top[u] = x[u][0];
-#pragma unroll
-      for (int i = 1; i < N; ++i) top[u] = fmaxf(top[u], x[u][i]);
-    }
-    float most = top[0];
-#pragma unroll
-    for (int u = 1; u < kVec; ++u) most = fmaxf(most, top[u]);
-    if (most > m + 32.f) {                             // the first tile; later ones only where terms could leave fp32's range
-      sum *= m == -INFINITY ? 0.f : ex2((m - most) * kLog2e);
-      m = most;
-    }
-    if (m > -INFINITY) {
-#pragma unroll
-      for (int u = 0; u < kVec; ++u)
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum += ex2((x[u][i] - m) * kLog2e);
-    } else {                                           // nothing but -infinity and NaN so far
-#pragma unroll
-      for (int u = 0; u < kVec; ++u)
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum += x[u][i] == -INFINITY ? 0.f : x[u][i];
-    }
-    if (first) {
-      first = false;
-      float gm = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
-      if ((lane & 3) == 0) s_group[tid >> 2] = gm;
-      __syncthreads();
-      if (tid < kGroups) {
-        const float own = s_group[tid];
-        int rank = 0;
-        for (int j = 0; j < kGroups; j += 4) {
-          const float4 o = *reinterpret_cast<const float4*>(&s_group[j]);
-          rank += (o.x > own || (o.x == own && j < tid)) + (o.y > own || (o.y == own && j + 1 < tid)) + (o.z > own || (o.z == own && j + 2 < tid)) +
-                  (o.w > own || (o.w == own && j + 3 < tid));
-        }
-        if (rank == n - 1) s_bound = own;
-      }
-      __syncthreads();
-      bound = s_bound;
-    }
-#pragma unroll
-    for (int u = 0; u < kVec; ++u) {
-      if (top[u] >= bound) {
-        const int64_t c0 = (t0 + u * kThreads + tid) * N - r.lead;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (x[u][i] >= bound && x[u][i] > -INFINITY) put_aside(x[u][i], c0 + i);
-      }
-    }
+__device__ __forceinline__ float top_of(const uint4& r) {
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&r);
+    const __nv_bfloat162 m = __hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3]));
+    return fmaxf(-INFINITY, fmaxf(__low2float(m), __high2float(m)));
+  } else {
+    const float* e = reinterpret_cast<const float*>(&r);
+    return fmaxf(fmaxf(fmaxf(-INFINITY, e[0]), e[1]), fmaxf(e[2], e[3]));
   }
-  // ---- the stretch's sum
-  const float mw = warp_max(m);
-  double part = m == -INFINITY ? (double)sum : (double)sum * exp((double)m - (double)mw);
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+// sums (a pair) += 2^(x log2 e - R) over a vector; c = (log2 e, log2 e), r = (-R, -R).
+template <typename T>
+__device__ __forceinline__ void add_exps(uint64_t& sums, const uint4& v, uint64_t c, uint64_t r) {
+  const unsigned e[4] = {v.x, v.y, v.z, v.w};
+  constexpr int PAIRS = Row<T>::N / 2;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-  if (lane == 0) { s_m[w] = mw; s_sum[w] = part; }
-  __syncthreads();
-  if (tid == 0) {
-    float mm = -INFINITY;
-    for (int i = 0; i < kThreads / 32; ++i) mm = fmaxf(mm, s_m[i]);
-    double all = 0.0;
-    for (int i = 0; i < kThreads / 32; ++i) all += s_m[i] == -INFINITY ? s_sum[i] : s_sum[i] * exp((double)s_m[i] - (double)mm);
-    parts[row * splits + split] = Part{all, mm, 0};
+  for (int i = 0; i < PAIRS; ++i) {
+    const uint64_t x = sizeof(T) == 2 ? pair_of(__uint_as_float(e[i] << 16), __uint_as_float(e[i] & 0xffff0000u))
+                                      : pair_of(__uint_as_float(e[2 * i % 4]), __uint_as_float(e[(2 * i + 1) % 4]));
+    uint64_t y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(y) : "l"(x), "l"(c), "l"(r));
+    float y0, y1;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(y0), "=f"(y1) : "l"(y));
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(sums) : "l"(sums), "l"(pair_of(ex2(y0), ex2(y1))));
   }
-  // ---- too many put aside: the n-th best of 128 groups of those kept is a higher bound.  At least 96 groups are below it, so that every
-  // pass leaves 1536 elements fewer; rows of one value or of a few allowed tokens take one, ascending ones as many as that says.
-  int count = s_count;
-  while (count > kCap) {
-    __syncthreads();
-    float gx = -INFINITY;
-    int gi = 0x7fffffff;
-    if (tid < kGroups) {
-      for (int j = tid; j < kCap; j += kGroups)
-        if (before(s_x[j], s_i[j], gx, gi)) { gx = s_x[j]; gi = s_i[j]; }
-      s_group[tid] = gx;
-      s_group_i[tid] = gi;
-    }
-    __syncthreads();
-    if (tid < kGroups) {
-      int rank = 0;
-      for (int j = 0; j < kGroups; ++j) rank += before(s_group[j], s_group_i[j], gx, gi);
-      if (rank == n - 1) { s_bound = gx; s_bound_i = gi; }
-    }
-    if (tid == 0) s_count = 0;
-    __syncthreads();
-    const float bx = s_bound;
-    const int bi = s_bound_i;
-    for (int64_t v = v0 + tid; v < v1; v += kThreads) {
-      float x[N];
-      r.load(v, x);
-      const int64_t c0 = v * N - r.lead;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (x[i] > bx || (x[i] == bx && c0 + i <= bi)) put_aside(x[i], c0 + i);
-    }
-    __syncthreads();
-    count = s_count;
-  }
-  // ---- the n best, sorted
-  float2* list = lists + (row * splits + split) * n;
-  for (int c = tid; c < count; c += kThreads) {
-    const float xc = s_x[c];
-    const int ic = s_i[c];
-    int rank = 0;
-    for (int j = 0; j < count; ++j) rank += before(s_x[j], s_i[j], xc, ic);
-    if (rank < n) list[rank] = make_float2(xc, __int_as_float(ic));
-  }
-  if (tid >= count && tid < n) list[tid] = make_float2(-INFINITY, __int_as_float(-1));      // fewer elements than that
+}
+__device__ __forceinline__ float sum_of(uint64_t p) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(p));
+  return a + b;
+}
+__device__ __forceinline__ double pow2(float e) {              // of a whole number from -1000 to 0, or less: zero
+  return e < -1000.f ? 0.0 : __hiloint2double((1023 + (int)e) << 20, 0);
 }
 
-// One CTA a sequence.  The n-th best of the lists' first entries bounds what can be among the n best of all; the few entries that reach it are ranked.
-// -infinity is nobody's list entry: where fewer than n candidates are above it, all of them have been selected, and the places left go
-// to the lowest k * V + t that have not.
-__global__ void __launch_bounds__(kThreads)
-beam_merge_kernel(int K, int V, int splits, const float* __restrict__ scores, const uint8_t* __restrict__ finished, int64_t pad, int n,
-                  const Part* __restrict__ parts, const float2* __restrict__ lists, float* __restrict__ out_scores, int32_t* __restrict__ out_parents,
-                  int64_t* __restrict__ out_tokens) {
-  constexpr int kMost = kMaxBest * (kMaxBest + 1);            // entries that can reach the bound
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ double s_val[kMost], s_bound;
-  __shared__ int64_t s_at[kMost], s_bound_at, s_taken[kMaxBest];
-  __shared__ int s_count;
-  double* lse = reinterpret_cast<double*>(smem);              // [K]
-  float2* s_list = reinterpret_cast<float2*>(lse + K);        // [K][splits][n]
-  pdl_launch_dependents();
-  const int64_t b = blockIdx.x;
-  const int tid = threadIdx.x, count = K * splits;
-  const float* score = scores + b * K;
-  const uint8_t* fin = finished ? finished + b * K : nullptr;
-  pdl_wait();
-  if (tid == 0) { s_count = 0; s_bound = -INFINITY; s_bound_at = INT64_MAX; }
-  for (int i = tid; i < count * n; i += kThreads) s_list[i] = __ldcg(&lists[b * count * n + i]);
-  for (int k = tid; k < K; k += kThreads) {
-    double l = __longlong_as_double(0x7ff8000000000000LL);    // not a number: the row has no candidates of its own
+// A value that the n-th largest of 64 groups' maxima reaches (x: this thread's maximum; a group: kThreads / 64 neighbours); -infinity where fewer than n
+// groups have one.  *most: the largest of all.  Groups are compared as whole numbers of the same order whose last six bits, taken off the
+// value, tell equal ones apart.  For all threads of the CTA; s: 64 words.
+__device__ __forceinline__ float nth_group(float x, int n, int* s, float* s_bound, float* most) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int o = 1; o < kThreads / kGroups; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  const int group = tid / (kThreads / kGroups), part = tid % (kThreads / kGroups);
+  const int bits = __float_as_int(x), order = bits ^ ((bits >> 31) & 0x7fffffff);
+  const int key = (order & ~(kGroups - 1)) | (kGroups - 1 - group);
+  if (part == 0) s[group] = key;
+  __syncthreads();
+  int rank = 0;
+  constexpr int PER = kGroups / (kThreads / kGroups);
+#pragma unroll
+  for (int j = 0; j < PER; j += 4) {
+    const int4 o = *reinterpret_cast<const int4*>(&s[part * PER + j]);
+    rank += (o.x > key) + (o.y > key) + (o.z > key) + (o.w > key);
+  }
+#pragma unroll
+  for (int o = 1; o < kThreads / kGroups; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+  const int down = order & ~(kGroups - 1);
+  if (rank == n - 1) s_bound[0] = x == -INFINITY ? -INFINITY : __int_as_float(down ^ ((down >> 31) & 0x7fffffff));
+  if (rank == 0) s_bound[1] = x;
+  __syncthreads();
+  *most = s_bound[1];
+  return s_bound[0];
+}
+
+// How many of s_x[0 .. count) (s_i: their places) come before entry e, counted by `per` neighbouring threads (a power of two up to 32).
+__device__ __forceinline__ int rank_of(const float* s_x, const int* s_i, int count, int e, int per) {
+  const float x = s_x[e];
+  const int at = s_i[e];
+  int rank = 0;
+  for (int j = threadIdx.x & (per - 1); j < count; j += per) rank += before(s_x[j], s_i[j], x, at);
+  for (int o = 1; o < per; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+  return rank;
+}
+// Threads per entry: as many as there are for all entries at once.
+__device__ __forceinline__ int threads_per(int count, int threads) {
+  int per = 1;
+  while (per < 32 && 2 * per * count <= threads) per *= 2;
+  return per;
+}
+
+struct RowsSmem {
+  float x[kCap];                                              // noted vectors: largest element, number; later the best ones' elements, columns
+  int i[kCap];
+  float y[kCap];                                              // those of them that reach a second bound
+  int j[kCap];
+};
+struct MergeSmem {
+  int64_t val[kMost], at[kMost], bound, bound_at, taken[kMaxBest];
+  double logsum[kMaxBeams];                                   // not a number where the row has no candidates of its own
+  float ref[kMaxBeams];                                       // logsumexp = ref + logsum
+  int count;
+};
+
+// Of one sequence, by the CTA that is done last: parts, list and what is behind them are this sequence's.  The n-th best of the lists' first entries
+// bounds what can be among the n best of all; the few entries that reach it are ranked.  -infinity is nobody's list entry: where fewer than n
+// candidates are above it, all of them have been selected, and the places left go to the lowest k * V + t that have not.
+__device__ __forceinline__ void merge(MergeSmem& s, int64_t b, int first_row, int K, int V, int splits, const float* __restrict__ score, const uint8_t* __restrict__ fin, int64_t pad,
+                                      int n, const Part* parts, const float2* list, float* __restrict__ out_scores,
+                                      int32_t* __restrict__ out_parents, int64_t* __restrict__ out_tokens) {
+  const int tid = threadIdx.x, lane = tid & 31, count = K * splits;
+  if (tid == 0) { s.count = 0; s.bound = INT64_MIN; s.bound_at = INT64_MAX; }
+  for (int k = tid >> 5; k < K; k += kThreads / 32) {             // a warp per row
+    double l = __longlong_as_double(0x7ff8000000000000LL);
+    float at = 0.f;
     if (score[k] > -INFINITY && !(fin && fin[k])) {
-      const Part* p = parts + (b * K + k) * splits;
-      float mm = -INFINITY;
-      for (int i = 0; i < splits; ++i) mm = fmaxf(mm, p[i].m);
+      const Part* p = parts + k * splits;
+      float R = -INFINITY, m = -INFINITY;
+      for (int i = lane; i < splits; i += 32) { R = fmaxf(R, __ldcg(&p[i].R)); m = fmaxf(m, __ldcg(&p[i].m)); }
+      R = warp_max(R);
+      m = warp_max(m);
       double all = 0.0;
-      for (int i = 0; i < splits; ++i) all += p[i].m == -INFINITY ? p[i].sum : p[i].sum * exp((double)p[i].m - (double)mm);
-      if (mm > -INFINITY && mm < INFINITY && all > 0.0) l = (double)mm + log(all);
+      for (int i = lane; i < splits; i += 32) {
+        const float Ri = __ldcg(&p[i].R);
+        const double f = R > -INFINITY ? (Ri > -INFINITY ? (R < INFINITY ? pow2(Ri - R) : 1.0) : 0.0) : __ldcg(&p[i].m) == m ? 1.0 : 0.0;
+        all += f * __ldcg(&p[i].sum);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+      if (R < INFINITY && all > 0.0) {
+        l = log(all) + (R > -INFINITY ? (double)R * (1.0 / (double)kLog2e) : 0.0);      // the log2 e that the sums were made with
+        at = R > -INFINITY ? 0.f : m;
+      }
     }
-    lse[k] = l;
+    if (lane == 0) { s.logsum[k] = l; s.ref[k] = at; }
   }
   __syncthreads();
-  auto entry = [&](int l, int pos, double& value, int64_t& at) {
+  // (value, beam << 32 | column); values as whole numbers of the same order: comparisons in 64-bit floating point take several times as long
+  auto entry = [&](int l, int pos, int64_t& order, int64_t& at) {
     const int k = l / splits;
-    value = -INFINITY;
+    double value = -INFINITY;
     at = INT64_MAX;
-    if (lse[k] == lse[k]) {
-      const float2 c = s_list[l * n + pos];
+    if (s.logsum[k] == s.logsum[k]) {
+      const float2 c = __ldcg(&list[l * n + pos]);
       const int col = __float_as_int(c.y);
-      if (col >= 0) { value = (double)score[k] + ((double)c.x - lse[k]); at = (int64_t)k * V + col; }
+      if (col >= 0) { value = (double)score[k] + (((double)c.x - (double)s.ref[k]) - s.logsum[k]); at = (int64_t)k << 32 | col; }
     } else if (fin && fin[k] && score[k] > -INFINITY && l % splits == 0 && pos == 0) {
       value = score[k];
-      at = (int64_t)k * V + pad;
+      at = (int64_t)k << 32 | pad;
     }
+    const int64_t bits = __double_as_longlong(value + 0.0);   // one zero
+    order = bits ^ ((bits >> 63) & INT64_MAX);
   };
-  auto first = [](double va, int64_t aa, double vb, int64_t ab) { return va > vb || (va == vb && aa < ab); };
-  const int depth = min(n, (n + count - 1) / count), heads = count * depth;      // heads <= max(count, 2 n): fits s_val
-  for (int i = tid; i < heads; i += kThreads) entry(i / depth, i % depth, s_val[i], s_at[i]);
+  auto first = [](int64_t va, int64_t aa, int64_t vb, int64_t ab) { return va > vb || (va == vb && aa < ab); };
+  const int depth = min(n, (n + count - 1) / count), heads = count * depth;      // heads <= max(count, 2 n): fits s.val
+  for (int i = tid; i < heads; i += kThreads) entry(i / depth, i % depth, s.val[i], s.at[i]);
   __syncthreads();
-  for (int i = tid; i < heads; i += kThreads) {
-    const double v = s_val[i];
-    const int64_t at = s_at[i];
-    if (at == INT64_MAX) continue;
+  auto rank_at = [&](int entries, int e, int per) {
+    const int64_t v = s.val[e], at = s.at[e];
     int rank = 0;
-    for (int j = 0; j < heads; ++j) rank += first(s_val[j], s_at[j], v, at);
-    if (rank == n - 1) { s_bound = v; s_bound_at = at; }
+    for (int j = tid & (per - 1); j < entries; j += per) rank += first(s.val[j], s.at[j], v, at);
+    for (int o = 1; o < per; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    return rank;
+  };
+  int per = threads_per(heads, kThreads);
+  for (int e0 = 0; e0 < heads; e0 += kThreads / per) {
+    const int e = e0 + tid / per, rank = rank_at(heads, min(e, heads - 1), per);
+    if (e < heads && rank == n - 1 && s.at[e] != INT64_MAX) { s.bound = s.val[e]; s.bound_at = s.at[e]; }
   }
   __syncthreads();
-  const double bound = s_bound;
-  const int64_t bound_at = s_bound_at;
+  const int64_t bound = s.bound, bound_at = s.bound_at;
   for (int i = tid; i < count * n; i += kThreads) {
-    double v;
-    int64_t at;
+    int64_t v, at;
     entry(i / n, i % n, v, at);
     if (at != INT64_MAX && !first(bound, bound_at, v, at)) {
-      const int slot = atomicAdd(&s_count, 1);
-      if (slot < kMost) { s_val[slot] = v; s_at[slot] = at; }
+      const int slot = atomicAdd(&s.count, 1);
+      if (slot < kMost) { s.val[slot] = v; s.at[slot] = at; }
     }
   }
   __syncthreads();
-  const int total = min(s_count, kMost);
-  for (int i = tid; i < total; i += kThreads) {
-    const double v = s_val[i];
-    const int64_t at = s_at[i];
-    int rank = 0;
-    for (int j = 0; j < total; ++j) rank += first(s_val[j], s_at[j], v, at);
-    if (rank < n) {
-      out_scores[b * n + rank] = (float)v;
-      out_parents[b * n + rank] = (int32_t)(b * K + at / V);
-      out_tokens[b * n + rank] = at % V;
-      s_taken[rank] = at;
+  const int total = min(s.count, kMost);
+  per = threads_per(total, kThreads);
+  for (int e0 = 0; e0 < total; e0 += kThreads / per) {
+    const int e = e0 + tid / per, rank = rank_at(total, min(e, total - 1), per);
+    if (e < total && rank < n && (tid & (per - 1)) == 0) {
+      const int64_t at = s.at[e];
+      const int64_t order = s.val[e];
+      out_scores[b * n + rank] = (float)__longlong_as_double(order ^ ((order >> 63) & INT64_MAX));
+      out_parents[b * n + rank] = first_row + (int32_t)(at >> 32);
+      out_tokens[b * n + rank] = at & 0xffffffffLL;
+      s.taken[rank] = at;
     }
   }
   if (total >= n) return;
   __syncthreads();
   if (tid == 0) {
-    int64_t at = 0;
-    for (int i = total; i < n; ++i, ++at) {
-      for (bool again = true; again;) {
-        again = false;
-        for (int j = 0; j < total; ++j)
-          if (s_taken[j] == at) { ++at; again = true; }
+    int k = 0, col = 0;
+    for (int i = total; i < n;) {
+      bool taken = false;
+      for (int j = 0; j < total; ++j) taken = taken || s.taken[j] == ((int64_t)k << 32 | col);
+      if (!taken) {
+        out_scores[b * n + i] = -INFINITY;
+        out_parents[b * n + i] = first_row + k;
+        out_tokens[b * n + i] = col;
+        ++i;
       }
-      out_scores[b * n + i] = -INFINITY;
-      out_parents[b * n + i] = (int32_t)(b * K + at / V);
-      out_tokens[b * n + i] = at % V;
+      if (++col == V) { col = 0; ++k; }                       // n <= K V: there are enough
     }
   }
 }
 
-// Stretches of a row: enough CTAs for four an SM, whole tiles of a CTA, and no more lists than the merge ranks in a microsecond or two.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 5)
+beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int V, int splits, int span, const float* __restrict__ scores,
+                   const uint8_t* __restrict__ finished, int64_t pad, int n, Part* parts, float2* lists, unsigned* __restrict__ counters,
+                   int first_row, float* __restrict__ out_scores, int32_t* __restrict__ out_parents, int64_t* __restrict__ out_tokens) {
+  constexpr int N = Row<T>::N, TILE = kThreads * kVec;
+  __shared__ __align__(16) uint8_t s_both[sizeof(RowsSmem) > sizeof(MergeSmem) ? sizeof(RowsSmem) : sizeof(MergeSmem)];
+  RowsSmem& rows = *reinterpret_cast<RowsSmem*>(s_both);
+  float (&s_x)[kCap] = rows.x, (&s_y)[kCap] = rows.y;
+  int (&s_i)[kCap] = rows.i, (&s_j)[kCap] = rows.j;
+  __shared__ bool s_mine;
+  __shared__ __align__(16) int s_group[kGroups];
+  __shared__ float s_bound[2], s_R[kThreads / 32], s_m[kThreads / 32], s_last;
+  __shared__ int s_best[kMaxBest], s_count, s_kept, s_elements;
+  __shared__ double s_sum[kThreads / 32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t row = blockIdx.x / splits;
+  const int split = (int)(blockIdx.x % splits), tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  // a row without a score or at its end has no candidates of its own
+  if (scores[row] > -INFINITY && !(finished && finished[row])) {
+  Row<T> r;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(logits + row * row_stride);
+  r.base = reinterpret_cast<const T*>(at & ~(uintptr_t)15);
+  r.lead = (int)((at & 15) / sizeof(T));
+  r.V = V;
+  const int vectors = (r.lead + V - 1) / N + 1;
+  const int v0 = split * span, v1 = min(vectors, v0 + span);
+  const int in0 = r.lead ? 1 : 0, in1 = (r.lead + V) / N;      // vectors that lie in the row as a whole
+  if (tid == 0) { s_count = s_kept = s_elements = 0; s_bound[0] = s_bound[1] = s_last = -INFINITY; }
+  auto note = [&](float x, int v) {
+    const int slot = atomicAdd(&s_count, 1);
+    if (slot < kCap) { s_x[slot] = x; s_i[slot] = v; }
+  };
+  const uint64_t c = pair_of(kLog2e, kLog2e);
+  uint64_t sums = pair_of(0.f, 0.f);
+  float R = -INFINITY, m = -INFINITY, bound = -INFINITY;       // m: with R = -infinity, the maximum, sums: how often
+  for (int t0 = v0; t0 < v1; t0 += TILE) {
+    uint4 x[kVec];
+    float top[kVec], most = -INFINITY;
+    if (t0 >= in0 && t0 + TILE <= min(v1, in1)) {
+      const uint4* p = reinterpret_cast<const uint4*>(r.base) + t0 + tid;
+#pragma unroll
+      for (int u = 0; u < kVec; ++u) x[u] = __ldcs(p + u * kThreads);
+    } else {
+      const float none = -INFINITY;
+      const unsigned word = sizeof(T) == 2 ? 0xff80ff80u : __float_as_uint(none);
+#pragma unroll
+      for (int u = 0; u < kVec; ++u) {
+        x[u] = make_uint4(word, word, word, word);
+        if (t0 + u * kThreads + tid < v1) x[u] = r.load(t0 + u * kThreads + tid);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kVec; ++u) {
+      top[u] = top_of<T>(x[u]);
+      most = fmaxf(most, top[u]);
+    }
+    if (t0 == v0) {
+      float ref;
+      bound = nth_group(most, n, s_group, s_bound, &ref);
+      if (ref > kLeast) R = ceilf(ref * kLog2e);
+    }
+    if (most > kLeast && most * kLog2e > R + 100.f) {         // terms could leave fp32's range, or are the first above kLeast
+      const float Rn = ceilf(most * kLog2e);
+      const float f = R == -INFINITY ? 0.f : ex2(R - Rn);
+      sums = pair_of(sum_of(sums) * f, 0.f);
+      R = Rn;
+    }
+    if (R > -INFINITY) {
+      const uint64_t minus = pair_of(-R, -R);
+#pragma unroll
+      for (int u = 0; u < kVec; ++u) add_exps<T>(sums, x[u], c, minus);
+    } else {
+      float count = sum_of(sums);
+#pragma unroll 1
+      for (int u = 0; u < kVec; ++u) {
+        alignas(16) T e[N];
+        *reinterpret_cast<uint4*>(e) = u == 0 ? x[0] : u == 1 ? x[1] : u == 2 ? x[2] : x[3];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float y = to_f32<T>(e[i]);
+          if (y > m) { m = y; count = count * 0.f + 1.f; }     // what is not a number stays so
+          else if (y == m) count += y == -INFINITY ? 0.f : 1.f;
+          else if (!(y < m)) count = y;
+        }
+      }
+      sums = pair_of(count, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < kVec; ++u)
+      if (top[u] >= bound && top[u] > -INFINITY) note(top[u], t0 + u * kThreads + tid);
+  }
+  // ---- the stretch's sum
+  {
+    const float Rw = warp_max(R), mw = warp_max(m);
+    if (lane == 0) { s_R[w] = Rw; s_m[w] = mw; }
+    __syncthreads();
+    float Rc = -INFINITY, mc = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) { Rc = fmaxf(Rc, s_R[i]); mc = fmaxf(mc, s_m[i]); }
+    double part = sum_of(sums);
+    if (Rc > -INFINITY) part *= R > -INFINITY ? (Rc < INFINITY ? pow2(R - Rc) : 1.0) : 0.0;
+    else part *= m == mc ? 1.0 : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    if (lane == 0) s_sum[w] = part;
+    __syncthreads();
+    if (tid == 0) {
+      double all = 0.0;
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) all += s_sum[i];
+      parts[row * splits + split] = Part{all, Rc, mc};
+    }
+  }
+  // ---- too many noted: the n-th of the threads' best among those kept (the larger element, then the lower number) is a higher bound.  n vectors reach it,
+  // and whatever the threads that come behind have kept, four vectors each, is left behind: the loop ends.
+  int count = s_count;
+  while (count > kCap) {
+    float bx = -INFINITY;
+    int bi = 0x7fffffff;
+    for (int j = tid; j < kCap; j += kThreads)
+      if (before(s_x[j], s_i[j], bx, bi)) { bx = s_x[j]; bi = s_i[j]; }
+    s_y[tid] = bx;
+    s_j[tid] = bi;
+    __syncthreads();
+    if (rank_of(s_y, s_j, kThreads, tid, 1) == n - 1) s_best[0] = tid;
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    bx = s_y[s_best[0]];
+    bi = s_j[s_best[0]];
+    for (int v = v0 + tid; v < v1; v += kThreads) {
+      const float top = top_of<T>(r.load(v));
+      if (top > bx || (top == bx && v <= bi)) note(top, v);
+    }
+    __syncthreads();
+    count = s_count;
+    __syncthreads();
+  }
+  // ---- a second bound on the noted vectors, if they are many; the n best of those that reach it, and of these the elements that reach the n-th
+  const bool many = count > kThreads / 4;
+  const float* noted_x = many ? s_y : s_x;
+  const int* noted_i = many ? s_j : s_i;
+  if (many) {
+    float most = -INFINITY, all;
+    for (int j = tid; j < count; j += kThreads) most = fmaxf(most, s_x[j]);
+    const float second = nth_group(most, n, s_group, s_bound, &all);
+    for (int j = tid; j < count; j += kThreads)
+      if (s_x[j] >= second) {
+        const int slot = atomicAdd(&s_kept, 1);
+        s_y[slot] = s_x[j];
+        s_j[slot] = s_i[j];
+      }
+    __syncthreads();
+    count = s_kept;
+  }
+  int per = threads_per(count, kThreads);
+  for (int e0 = 0; e0 < count; e0 += kThreads / per) {
+    const int e = e0 + tid / per, rank = rank_of(noted_x, noted_i, count, min(e, count - 1), per);
+    if (e < count && rank < n && (tid & (per - 1)) == 0) {
+      s_best[rank] = noted_i[e];
+      if (rank == n - 1) s_last = noted_x[e];                 // fewer vectors than that: every element of them
+    }
+  }
+  __syncthreads();
+  const int vecs = min(n, count);
+  if (tid < vecs * N) {                                       // at most 256
+    const int col = s_best[tid / N] * N - r.lead + tid % N;
+    const float x = col >= 0 && col < V ? to_f32<T>(r.base[r.lead + col]) : -INFINITY;
+    if (x >= s_last && x > -INFINITY) {
+      const int slot = atomicAdd(&s_elements, 1);
+      s_x[slot] = x;                                          // (noted vectors are done with: their numbers are in s_best)
+      s_i[slot] = col;
+    }
+  }
+  __syncthreads();
+  count = s_elements;
+  float2* list = lists + (row * splits + split) * n;
+  per = threads_per(count, kThreads);
+  if (count > 0) {
+    const int e = tid / per, rank = rank_of(s_x, s_i, count, min(e, count - 1), per);     // as many threads as entries, at least
+    if (e < count && rank < n && (tid & (per - 1)) == 0) list[rank] = make_float2(s_x[e], __int_as_float(s_i[e]));
+  }
+  if (tid >= count && tid < n) list[tid] = make_float2(-INFINITY, __int_as_float(-1));      // fewer elements than that
+  }
+  // ---- the sequence's last CTA merges
+  __syncthreads();
+  const int64_t b = row / K;
+  if (tid == 0) {
+    __threadfence();
+    const unsigned all = (unsigned)(K * splits);
+    s_mine = atomicInc(&counters[b], all - 1u) == all - 1u;   // back to zero with the last
+    __threadfence();
+  }
+  __syncthreads();
+  if (s_mine)
+    merge(*reinterpret_cast<MergeSmem*>(s_both), b, first_row + (int)(b * K), K, V, splits, scores + b * K, finished ? finished + b * K : nullptr, pad, n, parts + b * K * splits,
+          lists + b * K * splits * n, out_scores, out_parents, out_tokens);
+}
+
+// Stretches of a row: as many CTAs as the device holds (five an SM), whole tiles of a CTA, and no more lists than the merge ranks in a microsecond or two.
 int row_splits(int64_t rows, int K, int64_t V, int dtype) {
   const int64_t tile = kThreads * kVec * (dtype == TSB200_F32 ? 4 : 8);
-  int64_t s = (592 + rows - 1) / rows;
+  int64_t s = 740 / rows;
   const int64_t cap = (V + tile - 1) / tile, room = kMaxLists / K;
   if (s > cap) s = cap;
   if (s > room) s = room;
@@ -332,8 +478,8 @@ extern "C" {
 
 size_t tsb200_beam_select_workspace_bytes(int64_t B, int K, int64_t V, int dtype, int n) {
   if (B <= 0 || K <= 0 || V <= 0 || n <= 0) return 0;
-  const int64_t lists = B * K * row_splits(B * K, K, V, dtype);
-  return (size_t)(lists * (int64_t)(sizeof(Part) + n * sizeof(float2)) + 256);
+  const int64_t rows = (B < kCounters ? B : kCounters) * K, lists = rows * row_splits(rows, K, V, dtype);
+  return (size_t)(kCounters * sizeof(unsigned) + lists * (int64_t)(sizeof(Part) + n * sizeof(float2)));
 }
 
 int tsb200_beam_select(const void* logits, int dtype, int64_t row_stride, int64_t B, int K, int64_t V, const float* scores, const uint8_t* finished,
@@ -342,7 +488,7 @@ int tsb200_beam_select(const void* logits, int dtype, int64_t row_stride, int64_
   TSB_REQUIRE_DEVICE();
   if (B < 0 || K <= 0 || V <= 0 || n <= 0) return TSB200_ERR_ARG;
   if (dtype != TSB200_F32 && dtype != TSB200_BF16) return TSB200_ERR_UNSUPPORTED;
-  if (n > kMaxBest || K > kMaxBeams || V > 0x7fffffffLL - 64 || (int64_t)n > (int64_t)K * V) return TSB200_ERR_UNSUPPORTED;
+  if (n > kMaxBest || K > kMaxBeams || B * K > 0x7fffffffLL || V > 0x7fffffffLL - 65536 || (int64_t)n > (int64_t)K * V) return TSB200_ERR_UNSUPPORTED;
   const int64_t stride = row_stride ? row_stride : V;
   if (stride < V) return TSB200_ERR_ARG;
   if (finished && (pad_token < 0 || pad_token >= V)) return TSB200_ERR_ARG;
@@ -350,32 +496,26 @@ int tsb200_beam_select(const void* logits, int dtype, int64_t row_stride, int64_
   if (!logits || !scores || !out_scores || !out_parents || !out_tokens || !workspace || !aligned(workspace, 16)) return TSB200_ERR_ARG;
   if (!aligned(logits, dtype == TSB200_F32 ? 4 : 2)) return TSB200_ERR_ARG;
   if (workspace_bytes < tsb200_beam_select_workspace_bytes(B, K, V, dtype, n)) return TSB200_ERR_WORKSPACE;
-  const int splits = row_splits(B * K, K, V, dtype);
-  if (B * K > 0x7fffffffLL / splits || B > 0x7fffffffLL) return TSB200_ERR_UNSUPPORTED;
+  const int64_t step = B < kCounters ? B : kCounters;              // sequences of a launch
+  const int splits = row_splits(step * K, K, V, dtype);
+  if (step * K > 0x7fffffffLL / splits) return TSB200_ERR_UNSUPPORTED;
   const int per = dtype == TSB200_F32 ? 4 : 8;
   const int64_t vectors = (V + 2 * per - 2) / per;                 // a row may start inside a vector
-  const int64_t span = (vectors + splits - 1) / splits;
-  Part* parts = (Part*)workspace;
-  float2* lists = (float2*)(parts + B * K * splits);
-  cudaStream_t s = as_stream(stream);
-  const dim3 grid((unsigned)(B * K * splits));
-  if (dtype == TSB200_F32)
-    TSB_CUDA(launch_kernel(beam_rows_kernel<float>, grid, dim3(kThreads), 0, s, (const float*)logits, stride, (int)V, splits, span, scores, finished, n, parts,
-                           lists));
-  else
-    TSB_CUDA(launch_kernel(beam_rows_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, s, (const __nv_bfloat16*)logits, stride, (int)V, splits, span, scores,
-                           finished, n, parts, lists));
-  const size_t smem = (size_t)K * 8 + (size_t)K * splits * n * 8;
-  static bool configured[64] = {false};
-  int dev = 0;
-  TSB_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) return TSB200_ERR_DEVICE;
-  if (!configured[dev]) {
-    TSB_CUDA(cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBeams * 8 + kMaxLists * kMaxBest * 8));
-    configured[dev] = true;
+  const int span = (int)((vectors + splits - 1) / splits);
+  unsigned* counters = (unsigned*)workspace;
+  Part* parts = (Part*)(counters + kCounters);
+  float2* lists = (float2*)(parts + step * K * splits);
+  for (int64_t b = 0; b < B; b += step) {
+    const dim3 grid((unsigned)((B - b < step ? B - b : step) * K * splits));
+    const uint8_t* fin = finished ? finished + b * K : nullptr;
+    if (dtype == TSB200_F32)
+      TSB_CUDA(launch_kernel(beam_select_kernel<float>, grid, dim3(kThreads), 0, as_stream(stream), (const float*)logits + b * K * stride, stride, K, (int)V, splits, span,
+                             scores + b * K, fin, pad_token, n, parts, lists, counters, (int)(b * K), out_scores + b * n, out_parents + b * n, out_tokens + b * n));
+    else
+      TSB_CUDA(launch_kernel(beam_select_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, as_stream(stream), (const __nv_bfloat16*)logits + b * K * stride, stride, K,
+                             (int)V, splits, span, scores + b * K, fin, pad_token, n, parts, lists, counters, (int)(b * K), out_scores + b * n, out_parents + b * n,
+                             out_tokens + b * n));
   }
-  TSB_CUDA(launch_kernel_if(true, beam_merge_kernel, dim3((unsigned)B), dim3(kThreads), smem, s, K, (int)V, splits, scores, finished, pad_token, n, parts,
-                            lists, out_scores, out_parents, out_tokens));
   return TSB200_OK;
 }
 

@@ -402,7 +402,7 @@ class CompressedDecoder:
         scores = torch.full((B, K), float("-inf"), dtype=torch.float32, device=self.device)
         scores[:, 0] = 0.0
         finished = None if eos_token_id is None else torch.zeros((B, K), dtype=torch.bool, device=self.device)
-        ws = torch.empty(ops.beam_select_workspace_bytes(B, K, logits.shape[1], logits.dtype, K), dtype=torch.uint8, device=self.device)
+        ws = torch.zeros(ops.beam_select_workspace_bytes(B, K, logits.shape[1], logits.dtype, K), dtype=torch.uint8, device=self.device)
         new = torch.empty((B * K, max_new_tokens), dtype=torch.int64, device=self.device)
         for i in range(max_new_tokens):
             scores, parents, tokens = ops.beam_select(logits, scores, K, finished=finished, pad_token=pad or 0, ws=ws)

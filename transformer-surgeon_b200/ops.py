@@ -5,6 +5,8 @@ tensors, passes raw pointers plus the current stream to libtsb200.so and returns
 tensors.  No function has a CPU or eager-PyTorch fallback.
 """
 import ctypes as C
+import functools
+
 import torch
 
 from . import _lib
@@ -621,6 +623,7 @@ def prefill_attention(kv, q, L, sm_scale=None, out=None, status=None, seq_lens=N
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def decode_attn_workspace_bytes(B, H, head_dim, max_seq_len):
     return int(_lib.load().tsb200_paged_decode_attn_workspace_bytes(B, H, head_dim, max_seq_len))
 
@@ -665,7 +668,7 @@ def beam_select(logits, scores, n=None, finished=None, pad_token=0, out=None, ws
     logits [B * K, V] (or [B, K, V]; rows may be evenly strided), scores fp32 [B, K] of the beams: value = score + log_softmax(logits).  Returns
     (values fp32, parents int32, tokens int64), [B, n] each, best first, ties to the lower beam and token; a parent is a row of the batch
     (b * K + beam), as BeamReorder takes it.  finished: bool [B, K]; such a beam goes on as pad_token at its own score only.  A beam of score
-    -inf, or with a NaN or +inf among its logits, has no continuations; places without any are filled at -inf."""
+    -inf, or with a NaN or +inf among its logits, has no continuations; places without any are filled at -inf.  ws: zero-filled once, of one stream."""
     B, K = scores.shape
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor (this library has no CPU path)")
@@ -681,17 +684,21 @@ def beam_select(logits, scores, n=None, finished=None, pad_token=0, out=None, ws
     n = K if n is None else int(n)
     dt = _dt(logits)
     if out is None:
-        out = tuple(torch.empty((B, n), dtype=t, device=logits.device) for t in (torch.float32, torch.int32, torch.int64))
+        out = scores.new_empty((B, n)), scores.new_empty((B, n), dtype=torch.int32), scores.new_empty((B, n), dtype=torch.int64)
     elif any(o.shape != (B, n) or o.dtype != t for o, t in zip(out, (torch.float32, torch.int32, torch.int64))):
         raise ValueError("out must be float32, int32 and int64 tensors [B, n]")
     if ws is None:
         ws = workspace(logits.device, beam_select_workspace_bytes(B, K, V, logits.dtype, n), "beams")
-    stride = logits.stride(0) if B * K > 1 else V
-    check(_lib.load().tsb200_beam_select(_p(logits), dt, stride, B, K, V, _p(_cuda(scores, "scores")), 0 if finished is None else _p(_cuda(finished, "finished")),
-                                         int(pad_token), n, *(_p(_cuda(o, "out")) for o in out), _p(ws), ws.numel(), _stream()), "tsb200_beam_select")
+    values, parents, tokens = out
+    st = _lib.load().tsb200_beam_select(logits.data_ptr(), dt, logits.stride(0) if B * K > 1 else V, B, K, V, _cuda(scores, "scores").data_ptr(),
+                                        0 if finished is None else _cuda(finished, "finished").data_ptr(), int(pad_token), n, _cuda(values, "out").data_ptr(),
+                                        _cuda(parents, "out").data_ptr(), _cuda(tokens, "out").data_ptr(), ws.data_ptr(), ws.numel(), _stream())
+    if st:
+        check(st, "tsb200_beam_select")
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def beam_select_workspace_bytes(B, K, V, dtype, n):
     return int(_lib.load().tsb200_beam_select_workspace_bytes(B, K, V, F32 if dtype == torch.float32 else BF16, n))
 
