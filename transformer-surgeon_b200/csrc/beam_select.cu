@@ -15,7 +15,7 @@
 namespace tsb {
 namespace {
 
-constexpr int kThreads = 256, kVec = 4, kMaxBest = 32, kGroups = 64, kCap = 1024;
+constexpr int kThreads = 256, kVec = 4, kMaxBest = 32, kGroups = 64, kCap = 1024, kFew = 64;
 constexpr int kMaxLists = 256, kMaxBeams = 256;
 constexpr int kCounters = 4096;         // sequences of a launch; their counters are the workspace's head
 constexpr int kMost = kMaxBest * (kMaxBest + 1);            // entries that can reach the merge's bound
@@ -97,7 +97,7 @@ __device__ __forceinline__ double pow2(float e) {              // of a whole num
 // A value that the n-th largest of 64 groups' maxima reaches (x: this thread's maximum; a group: kThreads / 64 neighbours); -infinity where fewer than n
 // groups have one.  *most: the largest of all.  Groups are compared as whole numbers of the same order whose last six bits, taken off the
 // value, tell equal ones apart.  For all threads of the CTA; s: 64 words.
-__device__ __forceinline__ float nth_group(float x, int n, int* s, float* s_bound, float* most) {
+__device__ __noinline__ float nth_group(float x, int n, int* s, float* s_bound, float* most) {
   const int tid = threadIdx.x;
 #pragma unroll
   for (int o = 1; o < kThreads / kGroups; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -124,7 +124,7 @@ __device__ __forceinline__ float nth_group(float x, int n, int* s, float* s_boun
 }
 
 // How many of s_x[0 .. count) (s_i: their places) come before entry e, counted by `per` neighbouring threads (a power of two up to 32).
-__device__ __forceinline__ int rank_of(const float* s_x, const int* s_i, int count, int e, int per) {
+__device__ __noinline__ int rank_of(const float* s_x, const int* s_i, int count, int e, int per) {
   const float x = s_x[e];
   const int at = s_i[e];
   int rank = 0;
@@ -147,15 +147,16 @@ struct RowsSmem {
 };
 struct MergeSmem {
   int64_t val[kMost], at[kMost], bound, bound_at, taken[kMaxBest];
+  float least[kMaxBeams];                                     // logit below which a row's entries are below the bound
   double logsum[kMaxBeams];                                   // not a number where the row has no candidates of its own
   float ref[kMaxBeams];                                       // logsumexp = ref + logsum
   int count;
 };
 
-// Of one sequence, by the CTA that is done last: parts, list and what is behind them are this sequence's.  The n-th best of the lists' first entries
-// bounds what can be among the n best of all; the few entries that reach it are ranked.  -infinity is nobody's list entry: where fewer than n
+// Of one sequence, by the CTA that is done last: parts, list and what is behind them are this sequence's.  The lists' first entries bound what can be
+// among the n best of all; the few entries that reach the bound are ranked.  -infinity is nobody's list entry: where fewer than n
 // candidates are above it, all of them have been selected, and the places left go to the lowest k * V + t that have not.
-__device__ __forceinline__ void merge(MergeSmem& s, int64_t b, int first_row, int K, int V, int splits, const float* __restrict__ score, const uint8_t* __restrict__ fin, int64_t pad,
+__device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, int64_t b, int first_row, int K, int V, int splits, const float* __restrict__ score, const uint8_t* __restrict__ fin, int64_t pad,
                                       int n, const Part* parts, const float2* list, float* __restrict__ out_scores,
                                       int32_t* __restrict__ out_parents, int64_t* __restrict__ out_tokens) {
   const int tid = threadIdx.x, lane = tid & 31, count = K * splits;
@@ -165,15 +166,30 @@ __device__ __forceinline__ void merge(MergeSmem& s, int64_t b, int first_row, in
     float at = 0.f;
     if (score[k] > -INFINITY && !(fin && fin[k])) {
       const Part* p = parts + k * splits;
+      constexpr int U = 2;                                    // up to 64 parts on their way at once
       float R = -INFINITY, m = -INFINITY;
-      for (int i = lane; i < splits; i += 32) { R = fmaxf(R, __ldcg(&p[i].R)); m = fmaxf(m, __ldcg(&p[i].m)); }
-      R = warp_max(R);
-      m = warp_max(m);
       double all = 0.0;
-      for (int i = lane; i < splits; i += 32) {
-        const float Ri = __ldcg(&p[i].R);
-        const double f = R > -INFINITY ? (Ri > -INFINITY ? (R < INFINITY ? pow2(Ri - R) : 1.0) : 0.0) : __ldcg(&p[i].m) == m ? 1.0 : 0.0;
-        all += f * __ldcg(&p[i].sum);
+      for (int i0 = 0; i0 < splits; i0 += 32 * U) {
+        int4 raw[U];
+        float Rn = R, mn = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + 32 * u + lane;
+          raw[u] = i < splits ? __ldcg(reinterpret_cast<const int4*>(p + i)) : make_int4(0, 0, __float_as_int(-INFINITY), __float_as_int(-INFINITY));
+          Rn = fmaxf(Rn, __int_as_float(raw[u].z));
+          mn = fmaxf(mn, __int_as_float(raw[u].w));
+        }
+        Rn = warp_max(Rn);
+        mn = warp_max(mn);
+        // to the greater R: by a power of two; parts without one count where no part has one, for the greatest m
+        auto scaled = [&](double sum, float Ri, float mi) {
+          return sum * (Rn > -INFINITY ? (Ri > -INFINITY ? (Rn < INFINITY ? pow2(Ri - Rn) : 1.0) : 0.0) : mi == mn ? 1.0 : 0.0);
+        };
+        all = i0 ? scaled(all, R, m) : 0.0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) all += scaled(__hiloint2double(raw[u].y, raw[u].x), __int_as_float(raw[u].z), __int_as_float(raw[u].w));
+        R = Rn;
+        m = mn;
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
@@ -185,16 +201,17 @@ __device__ __forceinline__ void merge(MergeSmem& s, int64_t b, int first_row, in
     if (lane == 0) { s.logsum[k] = l; s.ref[k] = at; }
   }
   __syncthreads();
+  const float per_list = 1.f / n, per_row = 1.f / splits;      // quotients of at most 8192 by them, exact
   // (value, beam << 32 | column); values as whole numbers of the same order: comparisons in 64-bit floating point take several times as long
   auto entry = [&](int l, int pos, int64_t& order, int64_t& at) {
-    const int k = l / splits;
+    const int k = (int)((l + 0.5f) * per_row);
     double value = -INFINITY;
     at = INT64_MAX;
     if (s.logsum[k] == s.logsum[k]) {
       const float2 c = __ldcg(&list[l * n + pos]);
       const int col = __float_as_int(c.y);
       if (col >= 0) { value = (double)score[k] + (((double)c.x - (double)s.ref[k]) - s.logsum[k]); at = (int64_t)k << 32 | col; }
-    } else if (fin && fin[k] && score[k] > -INFINITY && l % splits == 0 && pos == 0) {
+    } else if (fin && fin[k] && score[k] > -INFINITY && l == k * splits && pos == 0) {
       value = score[k];
       at = (int64_t)k << 32 | pad;
     }
@@ -202,9 +219,7 @@ __device__ __forceinline__ void merge(MergeSmem& s, int64_t b, int first_row, in
     order = bits ^ ((bits >> 63) & INT64_MAX);
   };
   auto first = [](int64_t va, int64_t aa, int64_t vb, int64_t ab) { return va > vb || (va == vb && aa < ab); };
-  const int depth = min(n, (n + count - 1) / count), heads = count * depth;      // heads <= max(count, 2 n): fits s.val
-  for (int i = tid; i < heads; i += kThreads) entry(i / depth, i % depth, s.val[i], s.at[i]);
-  __syncthreads();
+  auto value_of = [](int64_t order) { return __longlong_as_double(order ^ ((order >> 63) & INT64_MAX)); };
   auto rank_at = [&](int entries, int e, int per) {
     const int64_t v = s.val[e], at = s.at[e];
     int rank = 0;
@@ -212,30 +227,80 @@ __device__ __forceinline__ void merge(MergeSmem& s, int64_t b, int first_row, in
     for (int o = 1; o < per; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
     return rank;
   };
-  int per = threads_per(heads, kThreads);
-  for (int e0 = 0; e0 < heads; e0 += kThreads / per) {
-    const int e = e0 + tid / per, rank = rank_at(heads, min(e, heads - 1), per);
-    if (e < heads && rank == n - 1 && s.at[e] != INT64_MAX) { s.bound = s.val[e]; s.bound_at = s.at[e]; }
-  }
-  __syncthreads();
-  const int64_t bound = s.bound, bound_at = s.bound_at;
-  for (int i = tid; i < count * n; i += kThreads) {
-    int64_t v, at;
-    entry(i / n, i % n, v, at);
-    if (at != INT64_MAX && !first(bound, bound_at, v, at)) {
-      const int slot = atomicAdd(&s.count, 1);
-      if (slot < kMost) { s.val[slot] = v; s.at[slot] = at; }
+  auto keep = [&](int64_t v, int64_t at) {
+    const int slot = atomicAdd(&s.count, 1);
+    if (slot < kMost) { s.val[slot] = v; s.at[slot] = at; }
+  };
+  // ---- a bound, the n-th largest of 64 groups, and the entries that reach it.  Neighbours are in groups of their own.
+  constexpr int U = 4, PER = kThreads / kGroups;
+  const int t0 = tid / PER + kGroups * (tid % PER);
+  float top = -INFINITY, all;
+  if (count * n <= U * kThreads) {                            // every entry
+    int64_t v[U], at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = t0 + u * kThreads, l = (int)((i + 0.5f) * per_list);
+      at[u] = INT64_MAX;
+      if (i < count * n) entry(l, i - l * n, v[u], at[u]);
+      if (at[u] != INT64_MAX) top = fmaxf(top, __double2float_rd(value_of(v[u])));
+    }
+    const double bound = nth_group(top, n, group, bound2, &all);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (at[u] != INT64_MAX && value_of(v[u]) >= bound) keep(v[u], at[u]);
+  } else {                                                    // the lists' first ones; they are more than n
+    for (int l = t0; l < count; l += kThreads) {
+      int64_t v, at;
+      entry(l, 0, v, at);
+      if (at != INT64_MAX) top = fmaxf(top, __double2float_rd(value_of(v)));
+    }
+    const float bound = nth_group(top, n, group, bound2, &all);
+    // the logit at which a row's entries reach it (within rounding: a few entries more do no harm)
+    if (tid < K) s.least[tid] = s.logsum[tid] == s.logsum[tid] ? __double2float_rd((double)bound - (double)score[tid] + s.logsum[tid] + (double)s.ref[tid]) : -INFINITY;
+    __syncthreads();
+    for (int i0 = tid; i0 < count * n; i0 += U * kThreads) {
+      float2 c[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) c[u] = i0 + u * kThreads < count * n ? __ldcg(&list[i0 + u * kThreads]) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kThreads, l = (int)((i + 0.5f) * per_list), k = (int)((l + 0.5f) * per_row);
+        if (i < count * n && (s.logsum[k] == s.logsum[k] ? c[u].x >= s.least[k] : l == k * splits && i == l * n)) {
+          int64_t v, at;
+          entry(l, i - l * n, v, at);
+          if (at != INT64_MAX) keep(v, at);
+        }
+      }
     }
   }
   __syncthreads();
+  if (s.count > kMost) {
+    // many equal values: the n-th best of the lists' first entries, lower columns first, leaves no more than n in each of n lists
+    __syncthreads();
+    if (tid == 0) s.count = 0;
+    const int depth = min(n, (n + count - 1) / count), heads = count * depth;    // heads <= max(count, 2 n): fits s.val
+    for (int i = tid; i < heads; i += kThreads) entry(i / depth, i % depth, s.val[i], s.at[i]);
+    __syncthreads();
+    for (int e = tid; e - tid < heads; e += kThreads) {
+      const int rank = rank_at(heads, min(e, heads - 1), 1);
+      if (e < heads && rank == n - 1 && s.at[e] != INT64_MAX) { s.bound = s.val[e]; s.bound_at = s.at[e]; }
+    }
+    __syncthreads();
+    const int64_t bound = s.bound, bound_at = s.bound_at;
+    for (int i = tid; i < count * n; i += kThreads) {
+      int64_t v, at;
+      entry(i / n, i % n, v, at);
+      if (at != INT64_MAX && !first(bound, bound_at, v, at)) keep(v, at);
+    }
+    __syncthreads();
+  }
   const int total = min(s.count, kMost);
-  per = threads_per(total, kThreads);
+  const int per = threads_per(total, kThreads);
   for (int e0 = 0; e0 < total; e0 += kThreads / per) {
     const int e = e0 + tid / per, rank = rank_at(total, min(e, total - 1), per);
     if (e < total && rank < n && (tid & (per - 1)) == 0) {
       const int64_t at = s.at[e];
-      const int64_t order = s.val[e];
-      out_scores[b * n + rank] = (float)__longlong_as_double(order ^ ((order >> 63) & INT64_MAX));
+      out_scores[b * n + rank] = (float)value_of(s.val[e]);
       out_parents[b * n + rank] = first_row + (int32_t)(at >> 32);
       out_tokens[b * n + rank] = at & 0xffffffffLL;
       s.taken[rank] = at;
@@ -388,7 +453,7 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
     if (rank_of(s_y, s_j, kThreads, tid, 1) == n - 1) s_best[0] = tid;
     if (tid == 0) s_count = 0;
     __syncthreads();
-    bx = s_y[s_best[0]];
+    bx = bound = s_y[s_best[0]];
     bi = s_j[s_best[0]];
     for (int v = v0 + tid; v < v1; v += kThreads) {
       const float top = top_of<T>(r.load(v));
@@ -398,48 +463,61 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
     count = s_count;
     __syncthreads();
   }
-  // ---- a second bound on the noted vectors, if they are many; the n best of those that reach it, and of these the elements that reach the n-th
-  const bool many = count > kThreads / 4;
-  const float* noted_x = many ? s_y : s_x;
-  const int* noted_i = many ? s_j : s_i;
-  if (many) {
+  // ---- a second bound on the noted vectors, if they are many; if it leaves many, the n best of them
+  const int* best = s_i;
+  if (count > kFew) {
     float most = -INFINITY, all;
     for (int j = tid; j < count; j += kThreads) most = fmaxf(most, s_x[j]);
-    const float second = nth_group(most, n, s_group, s_bound, &all);
+    bound = nth_group(most, n, s_group, s_bound, &all);
     for (int j = tid; j < count; j += kThreads)
-      if (s_x[j] >= second) {
+      if (s_x[j] >= bound) {
         const int slot = atomicAdd(&s_kept, 1);
         s_y[slot] = s_x[j];
         s_j[slot] = s_i[j];
       }
     __syncthreads();
     count = s_kept;
-  }
-  int per = threads_per(count, kThreads);
-  for (int e0 = 0; e0 < count; e0 += kThreads / per) {
-    const int e = e0 + tid / per, rank = rank_of(noted_x, noted_i, count, min(e, count - 1), per);
-    if (e < count && rank < n && (tid & (per - 1)) == 0) {
-      s_best[rank] = noted_i[e];
-      if (rank == n - 1) s_last = noted_x[e];                 // fewer vectors than that: every element of them
+    best = s_j;
+    if (count > kFew) {
+      for (int e = tid; e - tid < count; e += kThreads) {
+        const int rank = rank_of(s_y, s_j, count, min(e, count - 1), 1);
+        if (e < count && rank < n) {
+          s_best[rank] = s_j[e];
+          if (rank == n - 1) s_last = s_y[e];
+        }
+      }
+      __syncthreads();
+      count = n;
+      best = s_best;
+      bound = s_last;
     }
   }
-  __syncthreads();
-  const int vecs = min(n, count);
-  if (tid < vecs * N) {                                       // at most 256
-    const int col = s_best[tid / N] * N - r.lead + tid % N;
-    const float x = col >= 0 && col < V ? to_f32<T>(r.base[r.lead + col]) : -INFINITY;
-    if (x >= s_last && x > -INFINITY) {
+  // ---- their elements that reach the bound, and the n best of those, sorted
+  float x[2];
+  int col[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {                               // kFew vectors of 8 elements, at most
+    const int e = tid + u * kThreads;
+    x[u] = -INFINITY;
+    if (e < count * N) {
+      col[u] = best[e / N] * N - r.lead + e % N;
+      if (col[u] >= 0 && col[u] < V) x[u] = to_f32<T>(r.base[r.lead + col[u]]);
+    }
+  }
+  __syncthreads();                                            // the noted vectors are done with
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (x[u] >= bound && x[u] > -INFINITY) {
       const int slot = atomicAdd(&s_elements, 1);
-      s_x[slot] = x;                                          // (noted vectors are done with: their numbers are in s_best)
-      s_i[slot] = col;
+      s_x[slot] = x[u];
+      s_i[slot] = col[u];
     }
-  }
   __syncthreads();
   count = s_elements;
   float2* list = lists + (row * splits + split) * n;
-  per = threads_per(count, kThreads);
-  if (count > 0) {
-    const int e = tid / per, rank = rank_of(s_x, s_i, count, min(e, count - 1), per);     // as many threads as entries, at least
+  const int per = threads_per(count, kThreads);
+  for (int e0 = 0; e0 < count; e0 += kThreads / per) {
+    const int e = e0 + tid / per, rank = rank_of(s_x, s_i, count, min(e, count - 1), per);
     if (e < count && rank < n && (tid & (per - 1)) == 0) list[rank] = make_float2(s_x[e], __int_as_float(s_i[e]));
   }
   if (tid >= count && tid < n) list[tid] = make_float2(-INFINITY, __int_as_float(-1));      // fewer elements than that
@@ -455,7 +533,7 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
   }
   __syncthreads();
   if (s_mine)
-    merge(*reinterpret_cast<MergeSmem*>(s_both), b, first_row + (int)(b * K), K, V, splits, scores + b * K, finished ? finished + b * K : nullptr, pad, n, parts + b * K * splits,
+    merge(*reinterpret_cast<MergeSmem*>(s_both), s_group, s_bound, b, first_row + (int)(b * K), K, V, splits, scores + b * K, finished ? finished + b * K : nullptr, pad, n, parts + b * K * splits,
           lists + b * K * splits * n, out_scores, out_parents, out_tokens);
 }
 
