@@ -16,7 +16,7 @@ namespace tsb {
 namespace {
 
 constexpr int kThreads = 256, kVec = 4, kMaxBest = 32, kGroups = 64, kCap = 1024, kFew = 64;
-constexpr int kMaxLists = 256, kMaxBeams = 256;
+constexpr int kSlots = 592, kEntries = 4 * kThreads, kMaxBeams = 256;
 constexpr int kCounters = 4096;         // sequences of a launch; their counters are the workspace's head
 constexpr int kMost = kMaxBest * (kMaxBest + 1);            // entries that can reach the merge's bound
 constexpr float kLog2e = 1.4426950408889634f;
@@ -232,10 +232,10 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
     if (slot < kMost) { s.val[slot] = v; s.at[slot] = at; }
   };
   // ---- a bound, the n-th largest of 64 groups, and the entries that reach it.  Neighbours are in groups of their own.
-  constexpr int U = 4, PER = kThreads / kGroups;
+  constexpr int U = kEntries / kThreads, PER = kThreads / kGroups;
   const int t0 = tid / PER + kGroups * (tid % PER);
   float top = -INFINITY, all;
-  if (count * n <= U * kThreads) {                            // every entry
+  if (count * n <= kEntries) {                                // every entry
     int64_t v[U], at[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -325,7 +325,7 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 5)
+__global__ void __launch_bounds__(kThreads, 4)
 beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int V, int splits, int span, const float* __restrict__ scores,
                    const uint8_t* __restrict__ finished, int64_t pad, int n, Part* parts, float2* lists, unsigned* __restrict__ counters,
                    int first_row, float* __restrict__ out_scores, int32_t* __restrict__ out_parents, int64_t* __restrict__ out_tokens) {
@@ -537,11 +537,12 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
           lists + b * K * splits * n, out_scores, out_parents, out_tokens);
 }
 
-// Stretches of a row: as many CTAs as the device holds (five an SM), whole tiles of a CTA, and no more lists than the merge ranks in a microsecond or two.
-int row_splits(int64_t rows, int K, int64_t V, int dtype) {
+// Stretches of a row: as many CTAs as the device holds (four an SM), whole tiles of a CTA, and lists whose entries the merge takes in one step where that
+// leaves any choice (7 x 11 beams of 128256, n = 29: 9 stretches 30.9 us, 3 23.5).
+int row_splits(int64_t rows, int K, int64_t V, int dtype, int n) {
   const int64_t tile = kThreads * kVec * (dtype == TSB200_F32 ? 4 : 8);
-  int64_t s = 740 / rows;
-  const int64_t cap = (V + tile - 1) / tile, room = kMaxLists / K;
+  int64_t s = kSlots / rows;
+  const int64_t cap = (V + tile - 1) / tile, room = kEntries / ((int64_t)K * n);
   if (s > cap) s = cap;
   if (s > room) s = room;
   return (int)(s < 1 ? 1 : s);
@@ -556,7 +557,7 @@ extern "C" {
 
 size_t tsb200_beam_select_workspace_bytes(int64_t B, int K, int64_t V, int dtype, int n) {
   if (B <= 0 || K <= 0 || V <= 0 || n <= 0) return 0;
-  const int64_t rows = (B < kCounters ? B : kCounters) * K, lists = rows * row_splits(rows, K, V, dtype);
+  const int64_t rows = (B < kCounters ? B : kCounters) * K, lists = rows * row_splits(rows, K, V, dtype, n);
   return (size_t)(kCounters * sizeof(unsigned) + lists * (int64_t)(sizeof(Part) + n * sizeof(float2)));
 }
 
@@ -575,7 +576,7 @@ int tsb200_beam_select(const void* logits, int dtype, int64_t row_stride, int64_
   if (!aligned(logits, dtype == TSB200_F32 ? 4 : 2)) return TSB200_ERR_ARG;
   if (workspace_bytes < tsb200_beam_select_workspace_bytes(B, K, V, dtype, n)) return TSB200_ERR_WORKSPACE;
   const int64_t step = B < kCounters ? B : kCounters;              // sequences of a launch
-  const int splits = row_splits(step * K, K, V, dtype);
+  const int splits = row_splits(step * K, K, V, dtype, n);
   if (step * K > 0x7fffffffLL / splits) return TSB200_ERR_UNSUPPORTED;
   const int per = dtype == TSB200_F32 ? 4 : 8;
   const int64_t vectors = (V + 2 * per - 2) / per;                 // a row may start inside a vector
