@@ -139,10 +139,12 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
     if (w == 0) s_ends = 0u;
   }
   // Lengths and block table are inputs that the launch directly before this one does not write (see the header): looked up ahead of the wait.
+  // Where ranges end with sequences, a CTA counts its own alone.
+  const int each = (a.B + ranges - 1) / ranges, s0 = a.S ? 0 : min(range * each, a.B), s1 = a.S ? a.B : min(s0 + each, a.B);
   int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += NW * 32) {
+  for (int b0 = s0; b0 < s1; b0 += NW * 32) {
     const int b = b0 + (int)threadIdx.x;
-    int v = b < a.B ? pages_of(kv, b, a.max_seq_len) : 0;
+    int v = b < s1 ? pages_of(kv, b, a.max_seq_len) : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -156,21 +158,20 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
       if (i < w) v += s_scan[i];
       total += s_scan[i];
     }
-    if (b < a.B) cum[b] = before + v;
+    if (b < s1) cum[b] = before + v;
     before += total;
     __syncthreads();
   }
   const unsigned P = (unsigned)before;
-  auto start_of = [&](int b) { return (unsigned)(b ? cum[b - 1] : 0); };
+  auto start_of = [&](int b) { return (unsigned)(b > s0 ? cum[b - 1] : 0); };
   unsigned c0, c1, per = 0;
   if (a.S) {
     per = range_pages(P, ranges, a.per_min);
     c0 = min((uint64_t)P, (uint64_t)range * per);
     c1 = min((uint64_t)P, (uint64_t)c0 + per);
   } else {
-    const int each = (a.B + ranges - 1) / ranges, b0 = range * each, b1 = b0 + each;
-    c0 = b0 < a.B ? start_of(b0) : P;
-    c1 = b1 < a.B ? start_of(b1) : P;
+    c0 = 0;
+    c1 = P;
   }
   Cursor at;
   {
@@ -180,9 +181,9 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
     at.b = at.p = at.n = 0;
     if (at.left > 0) {
       // first sequence that ends behind x0: which 32, which of them
-      const int i0 = min(32 * lane + 31, a.B - 1);
-      int lo = 32 * (__ffs(__ballot_sync(0xffffffffu, (unsigned)cum[i0] > x0)) - 1);
-      lo += __ffs(__ballot_sync(0xffffffffu, (unsigned)cum[min(lo + lane, a.B - 1)] > x0)) - 1;
+      const int i0 = min(s0 + 32 * lane + 31, s1 - 1);
+      int lo = s0 + 32 * (__ffs(__ballot_sync(0xffffffffu, (unsigned)cum[i0] > x0)) - 1);
+      lo += __ffs(__ballot_sync(0xffffffffu, (unsigned)cum[min(lo + lane, s1 - 1)] > x0)) - 1;
       at.b = lo;
       at.p = (int)(x0 - start_of(lo));
       at.n = cum[lo] - (int)start_of(lo);
@@ -197,30 +198,30 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
     }
   };
 
-  // Lanes 0 and 1 copy K and V.  A page's number is looked up a round before its copies leave.
+  // Lanes 0 and 1 copy K and V.  Page numbers are looked up 32 at a time, one a lane.
   Cursor ahead = at;
-  int next_stage = 0;
-  const uint8_t* next_src = nullptr;
-  bool next = false;
+  int next_stage = 0, numbers = 0, first_number = 0, numbered = -1;       // of pages first_number .. of sequence `numbered`
   const int64_t rec_stride = (int64_t)kv.hkv * REC;
   const uint8_t* pool = (lane ? kv.v_pool : kv.k_pool) + (int64_t)hk * REC;
   auto look_up = [&]() {
-    next = ahead.left > 0;
-    if (next) {
-      if (lane < 2) {
-        const int page = kv.block_table[ahead.b * kv.bt_stride + ahead.p];
-        const int64_t pg = page < 0 ? 0 : (page >= kv.num_pages ? kv.num_pages - 1 : page);
-        next_src = pool + pg * rec_stride;
-      }
-      advance(ahead);
+    if (ahead.left > 0 && (ahead.b != numbered || ahead.p - first_number >= 32)) {
+      numbered = ahead.b;
+      first_number = ahead.p;
+      numbers = lane < ahead.n - ahead.p ? kv.block_table[ahead.b * kv.bt_stride + ahead.p + lane] : 0;
     }
   };
   auto issue = [&]() {
-    if (next) {
+    if (ahead.left > 0) {
+      const int page = __shfl_sync(0xffffffffu, numbers, ahead.p - first_number);
       if (lane == 0) mbar_expect_tx(&bars[next_stage], 2 * REC);
       __syncwarp();
-      if (lane < 2) bulk_g2s(ring + next_stage * C::STAGE + lane * REC, next_src, REC, &bars[next_stage]);
+      if (lane < 2) {
+        const int64_t pg = page < 0 ? 0 : (page >= kv.num_pages ? kv.num_pages - 1 : page);
+        bulk_g2s(ring + next_stage * C::STAGE + lane * REC, pool + pg * rec_stride, REC, &bars[next_stage]);
+      }
       next_stage = next_stage == kStages - 1 ? 0 : next_stage + 1;
+      advance(ahead);
+      look_up();
     }
   };
   // Elements of the column's query: 16 (tid + 4 c) + [0, 16)
@@ -249,10 +250,7 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
   pdl_wait();     // q and the newest token's pages come from the launches before
   if (at.left > 0) load_query(at.b);
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    issue();
-    look_up();
-  }
+  for (int i = 0; i < kStages - 1; ++i) issue();
 
   unsigned qf[D / 16][2];         // k-step 4 c + r: elements 16 (tid + 4 c) + 4 r + {0, 1}, {2, 3}
   float scf[2];                   // raw sum -> score in bits, of the heads whose scores this lane holds: 2 tid and 2 tid + 1, or tid
@@ -265,7 +263,6 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
 
   while (at.left > 0) {
     issue();
-    look_up();
     if (fresh) {
       if (!loaded) load_query(at.b);
       fresh = loaded = false;
@@ -498,9 +495,14 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
     }
   }
   // ---- sequences without tokens
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-    if (cum[b] == (int)start_of(b))
-      for (int i = threadIdx.x; i < a.H * D; i += NW * 32) out[(int64_t)b * a.H * D + i] = from_f32<T>(0.f);
+  for (int b = s0 + (a.S ? (int)blockIdx.x : 0); b < s1; b += a.S ? (int)gridDim.x : 1)
+    if (cum[b] == (int)start_of(b)) {
+      if (a.S) {                                             // of all heads; where ranges end with sequences, of the CTA's own
+        for (int i = threadIdx.x; i < a.H * D; i += NW * 32) out[(int64_t)b * a.H * D + i] = from_f32<T>(0.f);
+      } else {
+        for (int i = threadIdx.x; i < gn * D; i += NW * 32) out[((int64_t)b * a.H + hk * g + h0) * D + i] = from_f32<T>(0.f);
+      }
+    }
 }
 
 // One CTA per (sequence, head), one thread per element: adds up the parts of a sequence that crosses ranges, in order.  Chained to the attention.
