@@ -12,7 +12,7 @@
 // Work: the pages of all sequences in one row, cut into equal ranges, each for as many CTAs as there are kv heads, together as many as the device holds,
 // and each of those into equal ranges of its warps.  A warp streams its pages through a private ring (cp.async.bulk, K and V record) that does not
 // drain between sequences; a sequence that lies in one warp's range is done there, one that crosses warps is put together in shared memory
-// at the CTA's end, one that crosses ranges by a second launch.  So lengths of any mixture keep every SM busy to the end, and the heads of a page,
+// at the CTA's end, one that crosses ranges by a second launch (by the last of its CTAs: 5 us longer, one CTA then waits for every step of that alone).  So lengths of any mixture keep every SM busy to the end, and the heads of a page,
 // neighbours in memory, are read at about the same time (64 x 8192 tokens, 8 heads, pages in random order: 5.5 TB/s where they were not).
 #include "tc_common.cuh"
 #include "decode_attn_common.cuh"
