@@ -261,6 +261,58 @@ def test_attention_many_splits(cuda, name, B, hkv, g, d, L):
     assert torch.equal(out, ops.paged_decode_attention(kv, q, L))
 
 
+def test_attention_of_more_sequences_than_a_launch_takes(cuda):
+    from transformer_surgeon_b200 import ops
+    B, lens = 1100, [(37 * b) % 50 for b in range(1100)]
+    kv = make_kv(B, 4, 1, 64, cuda, lens=lens)
+    fill(kv, 50, 8)
+    q = torch.randn(B, 2, 64, generator=torch.Generator().manual_seed(6)).cuda()
+    ref, size = plain_attention(kv, q, lens, 0.125)
+    for longest in (50, 64):
+        out = ops.paged_decode_attention(kv, q, longest).double().cpu().numpy()
+        assert (np.abs(out - ref) <= tolerance("fp32", size, ref)).all()
+
+
+@pytest.mark.parametrize("B,L", [(2, 3000), (64, 700)])
+def test_attention_in_fixed_scratch(cuda, B, L):
+    """tsb200_paged_decode_attn_static: cut as far as the library's own scratch has room, whole sequences beyond that."""
+    import ctypes as C
+    from transformer_surgeon_b200 import _lib, ops
+    lens = [L - 7 * b for b in range(B)]
+    kv = make_kv(B, (L + 15) // 16, 8, 128, cuda, lens=lens)
+    fill(kv, L, 8)
+    q = torch.randn(B, 32, 128, generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+    out, desc = torch.empty_like(q), kv.desc()
+    for _ in range(2):
+        _lib.check(_lib.load().tsb200_paged_decode_attn_static(C.byref(desc), q.data_ptr(), out.data_ptr(), _lib.BF16, 32 * 128, B, 32, 128 ** -0.5, L,
+                                                               torch.cuda.current_stream().cuda_stream), "static")
+    ref, size = plain_attention(kv, q, lens, 128 ** -0.5)
+    assert (np.abs(out.double().cpu().numpy() - ref) <= tolerance("bf16", size, ref)).all()
+    assert torch.allclose(out.float(), ops.paged_decode_attention(kv, q, L).float(), rtol=2e-2, atol=2e-2)
+
+
+def test_attention_on_two_streams(cuda):
+    """Two calls at once, each with its own workspace and cache."""
+    from transformer_surgeon_b200 import ops
+    jobs = []
+    for i in range(2):
+        lens = [2000 - 300 * i - 11 * b for b in range(6)]
+        kv = make_kv(6, 125, 2, 64, cuda, seed=i, lens=lens)
+        fill(kv, 2000, 3 + i)
+        q = torch.randn(6, 8, 64, generator=torch.Generator().manual_seed(i)).cuda()
+        ws = torch.zeros(ops.decode_attn_workspace_bytes(6, 8, 64, 2000), dtype=torch.uint8, device=cuda)
+        jobs.append((kv, q, ws, torch.cuda.Stream(), ops.paged_decode_attention(kv, q, 2000, ws=ws).clone()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        outs = []
+        for kv, q, ws, stream, _ in jobs:
+            with torch.cuda.stream(stream):
+                outs.append(ops.paged_decode_attention(kv, q, 2000, ws=ws))
+        torch.cuda.synchronize()
+        for out, job in zip(outs, jobs):
+            assert torch.equal(out, job[4])
+
+
 def test_attention_pages_of_extreme_scales(cuda):
     """V scales 2^-40 and 2^40 in one sequence: weights and sums keep every page's share."""
     from transformer_surgeon_b200 import ops
@@ -575,6 +627,20 @@ def test_engine_beam_search_ends(cuda):
         dec.beam_search(ids, 60, 4)
 
 
+def test_blocks_path_with_pages_of_their_own_scales(cuda):
+    """The engine token by token against the prompt in one pass: no scales to set beforehand.  Logits a few e4m3 roundings (2^-4 of a value) apart,
+    as the pages' scales grow in other steps; within 2 % of the largest."""
+    _, a = tiny_engine(cuda, 2, "fp8_page")
+    _, b = tiny_engine(cuda, 2, "fp8_page")
+    ids = torch.randint(0, 512, (2, 21), generator=torch.Generator().manual_seed(5)).cuda()
+    one = a.prefill(ids).clone()
+    b.reset()
+    for t in range(21):
+        stepwise = b.step(ids[:, t])
+    assert (one - stepwise).abs().max() <= 2e-2 * one.abs().max()
+    assert torch.equal(a.seq_lens, b.seq_lens)
+
+
 @pytest.mark.parametrize("fmt", ["fp32", "fp8_page"])
 def test_hf_beam_search(cuda, fmt):
     """generate(num_beams=...) of Hugging Face over the paged cache: fp32 pages give the stock cache's sequences."""
@@ -663,6 +729,9 @@ def test_refusals(cuda):
     other = make_kv(2, 2, 1, 64, cuda)
     with pytest.raises(ValueError):
         ops.BeamReorder([kv, other])                              # another block table
+    many = make_kv(2049, 1, 1, 64, cuda)
+    with pytest.raises(ops.Tsb200Error):
+        ops.BeamReorder([many])(torch.zeros(2049, dtype=torch.int32, device=cuda))           # more rows than a CTA takes
     kv.block_table[1] = kv.block_table[0]
     with pytest.raises(ValueError):
         ops.BeamReorder([kv])                                     # rows without pages of their own

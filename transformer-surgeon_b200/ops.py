@@ -52,6 +52,13 @@ def _cuda(t, name):
     return t
 
 
+def _here(t, name):
+    """t on the current device: the call goes to that device's current stream."""
+    if t.device.index != _current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
+    return t
+
+
 def _token_strided(t, name):
     """t [B, T, heads, d] whose (heads, d) block is dense and whose tokens are evenly spaced
     (e.g. a column slice of a fused projection output).  Returns the token stride in elements."""
@@ -552,7 +559,7 @@ class BeamReorder:
     def __call__(self, parents, seq_lens=None):
         """parents int32 [rows]; a row whose parent is itself, out of range or of another length keeps what it has.  seq_lens: tokens cached per
         row, where that is not the first layer's tensor."""
-        rows, width = self.block_table.shape
+        rows, width = _here(self.block_table, "block_table").shape
         lens = self.seq_lens if seq_lens is None else _cuda(seq_lens, "seq_lens")
         if _cuda(parents, "parents").dtype != torch.int32 or parents.numel() != rows or lens.dtype != torch.int32 or lens.numel() != rows:
             raise ValueError(f"parents and seq_lens must be int32 [{rows}]")
@@ -672,6 +679,7 @@ def beam_select(logits, scores, n=None, finished=None, pad_token=0, out=None, ws
     B, K = scores.shape
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor (this library has no CPU path)")
+    _here(logits, "logits")
     if logits.dim() == 3:
         logits = logits.flatten(0, 1)
     V = logits.shape[1]
