@@ -9,7 +9,8 @@
 // bound, and the stretch is read once more; each such pass strictly raises it, and what is left does not depend on the order of the atomics.
 // The last CTA of a sequence to be done adds up the rows' sums, turns the sorted lists into values in 64 bits and merges them (a second launch, even
 // chained to the first, took 2 us longer, and 4 on the host).
-// Bound by the logits' bytes for many rows (the exponential unit needs three quarters of that time), by the chain of steps behind them for few.
+// Many rows: 32 x 8 beams of 152064 31 us, of which the bytes alone take 12, without exponentials 24.6, without what follows the noted vectors 26.3 (the next
+// tile requested ahead, or the bound raised again after 2, 4, 8 tiles: 31 and 32); few: the chain of steps behind the logits.
 #include "common.cuh"
 
 namespace tsb {
@@ -148,8 +149,8 @@ struct RowsSmem {
 struct MergeSmem {
   int64_t val[kMost], at[kMost], bound, bound_at, taken[kMaxBest];
   float least[kMaxBeams];                                     // logit below which a row's entries are below the bound
-  double logsum[kMaxBeams];                                   // not a number where the row has no candidates of its own
-  float ref[kMaxBeams];                                       // logsumexp = ref + logsum
+  double base[kMaxBeams];                                     // score - logsumexp + ref; not a number where the row has no candidates of its own
+  float ref[kMaxBeams];
   int count;
 };
 
@@ -161,6 +162,14 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
                                       int32_t* __restrict__ out_parents, int64_t* __restrict__ out_tokens) {
   const int tid = threadIdx.x, lane = tid & 31, count = K * splits;
   if (tid == 0) { s.count = 0; s.bound = INT64_MIN; s.bound_at = INT64_MAX; }
+  // entries, if they are few: neighbours in groups of their own; on their way while the rows' sums are made
+  constexpr int U = kEntries / kThreads, PER = kThreads / kGroups;
+  const int t0 = tid / PER + kGroups * (tid % PER);
+  float2 c[U];
+  if (count * n <= kEntries) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) c[u] = t0 + u * kThreads < count * n ? __ldcg(&list[t0 + u * kThreads]) : make_float2(-INFINITY, __int_as_float(-1));
+  }
   for (int k = tid >> 5; k < K; k += kThreads / 32) {             // a warp per row
     double l = __longlong_as_double(0x7ff8000000000000LL);
     float at = 0.f;
@@ -198,19 +207,19 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
         at = R > -INFINITY ? 0.f : m;
       }
     }
-    if (lane == 0) { s.logsum[k] = l; s.ref[k] = at; }
+    if (lane == 0) { s.base[k] = (double)score[k] - l; s.ref[k] = at; }
   }
   __syncthreads();
   const float per_list = 1.f / n, per_row = 1.f / splits;      // quotients of at most 8192 by them, exact
   // (value, beam << 32 | column); values as whole numbers of the same order: comparisons in 64-bit floating point take several times as long
-  auto entry = [&](int l, int pos, int64_t& order, int64_t& at) {
+  auto entry = [&](float2 c, int l, int pos, int64_t& order, int64_t& at) {
     const int k = (int)((l + 0.5f) * per_row);
+    const double base = s.base[k];
     double value = -INFINITY;
     at = INT64_MAX;
-    if (s.logsum[k] == s.logsum[k]) {
-      const float2 c = __ldcg(&list[l * n + pos]);
+    if (base == base) {
       const int col = __float_as_int(c.y);
-      if (col >= 0) { value = (double)score[k] + (((double)c.x - (double)s.ref[k]) - s.logsum[k]); at = (int64_t)k << 32 | col; }
+      if (col >= 0) { value = base + ((double)c.x - (double)s.ref[k]); at = (int64_t)k << 32 | col; }
     } else if (fin && fin[k] && score[k] > -INFINITY && l == k * splits && pos == 0) {
       value = score[k];
       at = (int64_t)k << 32 | pad;
@@ -231,9 +240,7 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
     const int slot = atomicAdd(&s.count, 1);
     if (slot < kMost) { s.val[slot] = v; s.at[slot] = at; }
   };
-  // ---- a bound, the n-th largest of 64 groups, and the entries that reach it.  Neighbours are in groups of their own.
-  constexpr int U = kEntries / kThreads, PER = kThreads / kGroups;
-  const int t0 = tid / PER + kGroups * (tid % PER);
+  // ---- a bound, the n-th largest of 64 groups, and the entries that reach it
   float top = -INFINITY, all;
   if (count * n <= kEntries) {                                // every entry
     int64_t v[U], at[U];
@@ -241,7 +248,7 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
     for (int u = 0; u < U; ++u) {
       const int i = t0 + u * kThreads, l = (int)((i + 0.5f) * per_list);
       at[u] = INT64_MAX;
-      if (i < count * n) entry(l, i - l * n, v[u], at[u]);
+      if (i < count * n) entry(c[u], l, i - l * n, v[u], at[u]);
       if (at[u] != INT64_MAX) top = fmaxf(top, __double2float_rd(value_of(v[u])));
     }
     const double bound = nth_group(top, n, group, bound2, &all);
@@ -251,23 +258,22 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
   } else {                                                    // the lists' first ones; they are more than n
     for (int l = t0; l < count; l += kThreads) {
       int64_t v, at;
-      entry(l, 0, v, at);
+      entry(__ldcg(&list[l * n]), l, 0, v, at);
       if (at != INT64_MAX) top = fmaxf(top, __double2float_rd(value_of(v)));
     }
     const float bound = nth_group(top, n, group, bound2, &all);
     // the logit at which a row's entries reach it (within rounding: a few entries more do no harm)
-    if (tid < K) s.least[tid] = s.logsum[tid] == s.logsum[tid] ? __double2float_rd((double)bound - (double)score[tid] + s.logsum[tid] + (double)s.ref[tid]) : -INFINITY;
+    if (tid < K) s.least[tid] = s.base[tid] == s.base[tid] ? __double2float_rd((double)bound - s.base[tid] + (double)s.ref[tid]) : -INFINITY;
     __syncthreads();
     for (int i0 = tid; i0 < count * n; i0 += U * kThreads) {
-      float2 c[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) c[u] = i0 + u * kThreads < count * n ? __ldcg(&list[i0 + u * kThreads]) : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + u * kThreads, l = (int)((i + 0.5f) * per_list), k = (int)((l + 0.5f) * per_row);
-        if (i < count * n && (s.logsum[k] == s.logsum[k] ? c[u].x >= s.least[k] : l == k * splits && i == l * n)) {
+        if (i < count * n && (s.base[k] == s.base[k] ? c[u].x >= s.least[k] : l == k * splits && i == l * n)) {
           int64_t v, at;
-          entry(l, i - l * n, v, at);
+          entry(c[u], l, i - l * n, v, at);
           if (at != INT64_MAX) keep(v, at);
         }
       }
@@ -279,7 +285,7 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
     __syncthreads();
     if (tid == 0) s.count = 0;
     const int depth = min(n, (n + count - 1) / count), heads = count * depth;    // heads <= max(count, 2 n): fits s.val
-    for (int i = tid; i < heads; i += kThreads) entry(i / depth, i % depth, s.val[i], s.at[i]);
+    for (int i = tid; i < heads; i += kThreads) entry(__ldcg(&list[i / depth * n + i % depth]), i / depth, i % depth, s.val[i], s.at[i]);
     __syncthreads();
     for (int e = tid; e - tid < heads; e += kThreads) {
       const int rank = rank_at(heads, min(e, heads - 1), 1);
@@ -289,7 +295,7 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
     const int64_t bound = s.bound, bound_at = s.bound_at;
     for (int i = tid; i < count * n; i += kThreads) {
       int64_t v, at;
-      entry(i / n, i % n, v, at);
+      entry(__ldcg(&list[i]), i / n, i % n, v, at);
       if (at != INT64_MAX && !first(bound, bound_at, v, at)) keep(v, at);
     }
     __syncthreads();
@@ -361,22 +367,24 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
   const uint64_t c = pair_of(kLog2e, kLog2e);
   uint64_t sums = pair_of(0.f, 0.f);
   float R = -INFINITY, m = -INFINITY, bound = -INFINITY;       // m: with R = -infinity, the maximum, sums: how often
-  for (int t0 = v0; t0 < v1; t0 += TILE) {
-    uint4 x[kVec];
-    float top[kVec], most = -INFINITY;
+  auto load_tile = [&](int t0, uint4 (&x)[kVec]) {
     if (t0 >= in0 && t0 + TILE <= min(v1, in1)) {
       const uint4* p = reinterpret_cast<const uint4*>(r.base) + t0 + tid;
 #pragma unroll
       for (int u = 0; u < kVec; ++u) x[u] = __ldcs(p + u * kThreads);
     } else {
-      const float none = -INFINITY;
-      const unsigned word = sizeof(T) == 2 ? 0xff80ff80u : __float_as_uint(none);
+      const unsigned word = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;         // -infinity
 #pragma unroll
       for (int u = 0; u < kVec; ++u) {
         x[u] = make_uint4(word, word, word, word);
         if (t0 + u * kThreads + tid < v1) x[u] = r.load(t0 + u * kThreads + tid);
       }
     }
+  };
+  for (int t0 = v0; t0 < v1; t0 += TILE) {
+    uint4 x[kVec];
+    load_tile(t0, x);
+    float top[kVec], most = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kVec; ++u) {
       top[u] = top_of<T>(x[u]);
@@ -493,23 +501,23 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
     }
   }
   // ---- their elements that reach the bound, and the n best of those, sorted
-  float x[2];
+  float y[2];
   int col[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {                               // kFew vectors of 8 elements, at most
     const int e = tid + u * kThreads;
-    x[u] = -INFINITY;
+    y[u] = -INFINITY;
     if (e < count * N) {
       col[u] = best[e / N] * N - r.lead + e % N;
-      if (col[u] >= 0 && col[u] < V) x[u] = to_f32<T>(r.base[r.lead + col[u]]);
+      if (col[u] >= 0 && col[u] < V) y[u] = to_f32<T>(r.base[r.lead + col[u]]);
     }
   }
   __syncthreads();                                            // the noted vectors are done with
 #pragma unroll
   for (int u = 0; u < 2; ++u)
-    if (x[u] >= bound && x[u] > -INFINITY) {
+    if (y[u] >= bound && y[u] > -INFINITY) {
       const int slot = atomicAdd(&s_elements, 1);
-      s_x[slot] = x[u];
+      s_x[slot] = y[u];
       s_i[slot] = col[u];
     }
   __syncthreads();
