@@ -7,8 +7,8 @@
 // stretch's n best.  What "can still be" means: the n-th largest of 64 group maxima of the first tile, a value that n elements reach.  At the end the n
 // best of the noted vectors hold the n best elements; those alone are looked at one by one.  More noted vectors than there is room for raise the
 // bound, and the stretch is read once more; each such pass strictly raises it, and what is left does not depend on the order of the atomics.
-// The last CTA of a sequence to be done adds up the rows' sums, turns the sorted lists into values in 64 bits and merges them (a second launch, even
-// chained to the first, took 2 us longer, and 4 on the host).
+// The last CTA of a sequence to be done adds up the rows' sums, turns the sorted lists into values in 64 bits and merges them (as a second launch, chained to
+// the first, about as long on the device and 4 us more of the host's time a call).
 // Many rows: 32 x 8 beams of 152064 31 us, of which the bytes alone take 12, without exponentials 24.6, without what follows the noted vectors 26.3 (the next
 // tile requested ahead, or the bound raised again after 2, 4, 8 tiles: 31 and 32); few: the chain of steps behind the logits.
 #include "common.cuh"

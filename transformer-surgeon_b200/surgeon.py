@@ -186,7 +186,7 @@ def decoder_from_model(model, batch=1, max_seq_len=None, kv_format=None, device=
 
     options: the dict `convert_for_export` takes (utils/convert.py:304-308): `max_cache_len` (default 2048)
     bounds the context, `cache_impl` picks the cache format among blocks_path.CACHE_IMPLS (`paged_int8`,
-    `paged_fp8`, `paged_nvfp4`, `paged_bf16`, `paged_fp32`); `use_sdpa` has no meaning here.  Explicit
+    `paged_fp8`, `paged_nvfp4`, `paged_bf16`, `paged_fp32`, `paged_fp8_page`); `use_sdpa` has no meaning here.  Explicit
     `max_seq_len` / `kv_format` arguments win over the options.  The layer math is the HF model's (what
     `generate()` runs); for the reference's blocks-path variant of the math use `convert_for_export`."""
     from . import blocks_path
