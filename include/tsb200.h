@@ -64,7 +64,7 @@ int tsb200_check_device(void);
  * returns the previous setting.  Default 0.
  * What a kernel touches before that ordering point is constant data (weights, weight and cache scales, RoPE tables),
  * the lengths and the block table (seq_lens, new_lens, block_table: read by the append and by the decode attention) and,
- * in the FP8 decode attention with one split, pages of the cache STRICTLY OLDER than the one that holds a sequence's
+ * in the FP8 decode attention with one split and in that of FP8_PAGE, pages of the cache STRICTLY OLDER than the one that holds a sequence's
  * newest token.  With this setting on, the launch that directly precedes an append or a decode attention on its stream
  * must therefore not be the one that writes those: advance lengths, remap pages and refresh scales at least two launches
  * ahead (the engine of this package does so at the start of a step), or turn the setting off around such a pair, or (decode attention)

@@ -583,7 +583,7 @@ def tiny_engine(cuda, batch, kv_format, dtype=torch.float32):
 
 
 @pytest.mark.parametrize("captured", [False, True])
-@pytest.mark.parametrize("kv_format", ["fp32", "fp8_page"])
+@pytest.mark.parametrize("kv_format", ["fp32", "fp8_page", "fp8", "int8"])
 def test_engine_beam_search(cuda, captured, kv_format):
     """CompressedDecoder.beam_search against a search that feeds every beam's whole sequence to a fresh cache each step."""
     B, K, T, new = 2, 3, 9, 12
@@ -606,6 +606,22 @@ def test_engine_beam_search(cuda, captured, kv_format):
         rows = torch.cat((rows.view(B, K, -1).gather(1, (at // 512)[..., None].expand(B, K, rows.shape[1])), (at % 512)[..., None]), 2).flatten(0, 1)
     assert torch.equal(rows.view(B, K, -1), seqs)
     assert torch.allclose(total.float(), scores, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("kv_format,dtype", [("fp8_page", torch.bfloat16), ("nvfp4", torch.bfloat16), ("fp8", torch.float32)])
+@pytest.mark.parametrize("T", [1, 16, 37])
+def test_prompt_once_for_all_beams(cuda, kv_format, dtype, T):
+    """The rows of a prompt hold what each holds that went through the model by itself, up to the order of sums in layers of other token counts."""
+    _, a = tiny_engine(cuda, 6, kv_format, dtype)
+    _, b = tiny_engine(cuda, 6, kv_format, dtype)
+    ids = torch.randint(0, 512, (2, T), generator=torch.Generator().manual_seed(5)).cuda()
+    one, each = a.prefill(ids, beams=3).clone(), b.prefill(ids.repeat_interleave(3, 0)).clone()
+    tol = 2e-2 if dtype == torch.bfloat16 else 2e-3
+    for _ in range(3):
+        assert (one - each).abs().max() <= tol * each.abs().max()
+        tokens = each.argmax(-1)
+        one, each = a.step(tokens).clone(), b.step(tokens).clone()
+    assert torch.equal(a.seq_lens, b.seq_lens)
 
 
 def test_engine_beam_search_ends(cuda):

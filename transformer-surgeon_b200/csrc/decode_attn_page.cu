@@ -247,10 +247,12 @@ decode_attn_page_kernel(tsb200_kv_desc kv, const T* __restrict__ q, PageArgs a, 
       }
   };
   look_up();
+  // Pages strictly older than a sequence's newest are written by no append before this launch: their copies leave while those launches finish.
+  int started = 0;
+  for (; started < kStages - 1 && ahead.left > 0 && ahead.p + 1 < ahead.n; ++started) issue();
   pdl_wait();     // q and the newest token's pages come from the launches before
   if (at.left > 0) load_query(at.b);
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue();
+  for (; started < kStages - 1; ++started) issue();
 
   unsigned qf[D / 16][2];         // k-step 4 c + r: elements 16 (tid + 4 c) + 4 r + {0, 1}, {2, 3}
   float scf[2];                   // raw sum -> score in bits, of the heads whose scores this lane holds: 2 tid and 2 tid + 1, or tid

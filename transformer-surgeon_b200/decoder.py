@@ -327,31 +327,48 @@ class CompressedDecoder:
             raise ops.Tsb200Error(ops._lib.ERR_TIMEOUT, "a bounded device-side wait ran out: " +
                                   ", ".join(f"{k} status {v}" for k, v in bad.items()))
 
+    def _first_rows(self, beams):
+        """The caches of every beams-th row."""
+        table, lens, views = self.block_table[::beams].contiguous(), self.seq_lens[::beams].contiguous(), []
+        for kv in self.kv:
+            view = ops.PagedKV.__new__(ops.PagedKV)
+            view.__dict__.update(kv.__dict__)
+            view.block_table, view.seq_lens = table, lens
+            if kv.k_scale is not None:
+                view.k_scale, view.v_scale = kv.k_scale[::beams].contiguous(), kv.v_scale[::beams].contiguous()
+            views.append(view)
+        return views
+
     @torch.no_grad()
-    def prefill(self, input_ids):
+    def prefill(self, input_ids, beams=1):
         """Batched prompt pass (single GPU): all T prompt tokens of every sequence go through the packed
         linears at once (M = B * T rows), K and V are rotated, quantized and appended for the whole chunk
         (FP8: the per-sequence scales are taken over the prompt first, amax / 448, and then frozen), and the
         causal attention of the chunk reads the DEQUANTIZED cache: bf16 engines on the tcgen05 prefill kernel
         (`tsb200_kv_gather_heads` + `tsb200_prefill_attn`), fp32 engines on the paged decode kernel with one
         one-token "sequence" per query.  Leaves the engine in the state the token-by-token prompt loop leaves it
-        in: logits / next_tokens of the last prompt token, seq_lens == T.  Starts from an empty cache."""
+        in: logits / next_tokens of the last prompt token, seq_lens == T.  Starts from an empty cache.
+        beams: rows of the engine per prompt (input_ids [batch / beams, T]): the prompts go through the model once, their pages are shared by the
+        rows, and every row has its prompt's logits."""
         c = self.cfg
         if c.tp_world > 1:
             raise NotImplementedError("batched prefill is single-GPU; tensor-parallel engines feed the prompt stepwise")
         ids = input_ids.to(self.device)
         B, T = ids.shape
-        if B != self.B or T < 1 or T > self.max_seq_len:
+        if B * beams != self.B or T < 1 or T > self.max_seq_len:
             raise ValueError("prompt does not fit the engine")
         H, Hkv, d = self.H_local, self.Hkv_local, c.head_dim
+        if beams > 1 and self._beams is None:
+            self._beams = ops.BeamReorder(self.kv)
         self.reset()
-        zeros = torch.zeros_like(self.seq_lens)
+        zeros = self.seq_lens.new_zeros(B)
         rope = (self.cos, self.sin)
         resid = self.embed[ids.reshape(-1)].contiguous()                # [B*T, hidden]
         delta = None
         self.seq_lens.fill_(T)                                          # appends take their positions from `zeros`
         status = self.attn_ws[ops.ATTN_STATUS_OFFSET:ops.ATTN_STATUS_OFFSET + 4]
-        sequences = ops.query_sequences(self.kv[0], B, T, T, self.seq_lens) if c.dtype == torch.float32 else None
+        caches = self.kv if beams == 1 else self._first_rows(beams)
+        sequences = ops.query_sequences(caches[0], B, T, T) if c.dtype == torch.float32 else None
         for li, L in enumerate(self.layers):
             xn = ops.add_rmsnorm(resid, delta, L.ln1, c.rms_eps, c.norm_variant)
             if L.qkv is not None:
@@ -362,17 +379,22 @@ class CompressedDecoder:
             else:
                 q, k, v = L.qkv_group(xn)
                 q4, k4, v4 = q.view(B, T, H, d), k.view(B, T, Hkv, d), v.view(B, T, Hkv, d)
-            kv = self.kv[li]
+            kv = caches[li]
             if kv.k_scale is not None:
                 kv.set_fp8_scales(k4, v4, rope=rope, pos0=zeros)
+                if beams > 1:
+                    self.kv[li].fill_fp8_scales(kv.k_scale.repeat_interleave(beams, 0), kv.v_scale.repeat_interleave(beams, 0))
             kv.rope_append(q4, k4, v4, rope, seq_lens=zeros)            # q4 rotated in place
             # causal attention of the chunk over the DEQUANTIZED cache (what every attention read sees)
             att = ops.prefill_attention(kv, q4, T, status=status, sequences=sequences)
             delta = L.o(att.view(B * T, H * d))
             xn = ops.add_rmsnorm(resid, delta, L.ln2, c.rms_eps, c.norm_variant)
             delta = L.mlp(xn)
-        last = resid.view(B, T, -1)[:, -1].contiguous()
-        dl = delta.view(B, T, -1)[:, -1].contiguous()
+        if beams > 1:                                                   # every row takes over its prompt's first row
+            rows = torch.arange(self.B, dtype=torch.int32, device=self.device)
+            self._beams(rows - rows % beams, self.seq_lens)
+        last = resid.view(B, T, -1)[:, -1].repeat_interleave(beams, 0)
+        dl = delta.view(B, T, -1)[:, -1].repeat_interleave(beams, 0)
         self.resid.copy_(last)
         ops.add_rmsnorm(self.resid, dl, self.final_norm, c.rms_eps, c.norm_variant, out=self.xn)
         self.lm_head(self.xn, out=self.logits, ws=self.lin_ws)
@@ -384,7 +406,7 @@ class CompressedDecoder:
         """Beam search over input_ids [B, T] on an engine built for B * num_beams sequences: every step keeps the num_beams best continuations
         of a sequence by their summed log probabilities, and the caches follow them (full pages are shared between beams).  With eos_token_id a
         beam that ends stays as it is, padded with pad_token_id (default: eos_token_id).  Returns (sequences int64 [B, num_beams, T + max_new_tokens],
-        scores fp32 [B, num_beams]), best first.  The prompt goes through prefill()."""
+        scores fp32 [B, num_beams]), best first.  The prompts go through prefill(), once for all their beams."""
         ids = input_ids.to(self.device)
         B, T = ids.shape
         K = int(num_beams)
@@ -395,9 +417,9 @@ class CompressedDecoder:
         if max_new_tokens < 1 or T + max_new_tokens - 1 > self.max_seq_len:
             raise ValueError("prompt and new tokens do not fit the engine")
         pad = eos_token_id if pad_token_id is None else pad_token_id
-        if self._beams is None:
+        logits = self.prefill(ids, beams=K)
+        if self._beams is None:                                          # one beam
             self._beams = ops.BeamReorder(self.kv)
-        logits = self.prefill(ids.repeat_interleave(K, dim=0))
         # all beams are one beam at first: the others have no continuations yet
         scores = torch.full((B, K), float("-inf"), dtype=torch.float32, device=self.device)
         scores[:, 0] = 0.0
