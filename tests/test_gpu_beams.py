@@ -722,6 +722,45 @@ def test_select_and_reorder_captured(cuda):
         assert torch.equal(beside[2], ops.beam_select(other, torch.zeros(3, R, device=cuda), 2)[2])
 
 
+def test_default_scratch_is_of_one_stream_and_of_one_graph(cuda):
+    """Selection and attention without a workspace: on two streams at once, in two graphs replayed at once, and eagerly after a capture that never ran."""
+    from transformer_surgeon_b200 import ops
+    jobs = []
+    for i, (B, K, V) in enumerate(((5, 4, 70001), (2, 7, 90002))):
+        kv = make_kv(B * K, 40, 1, 64, cuda, seed=i, lens=[600 - 17 * r for r in range(B * K)])
+        fill(kv, 600, i)
+        g = torch.Generator().manual_seed(i)
+        args = torch.randn(B * K, V, generator=g).to(cuda), torch.randn(B, K, generator=g).to(cuda), kv, torch.randn(B * K, 8, 64, generator=g).to(cuda)
+        ws = [torch.zeros(n, dtype=torch.uint8, device=cuda)
+              for n in (ops.beam_select_workspace_bytes(B, K, V, torch.float32, K), ops.decode_attn_workspace_bytes(B * K, 8, 64, 640))]
+
+        def run(args=args, ws=(None, None)):
+            logits, scores, kv, q = args
+            return (*ops.beam_select(logits, scores, ws=ws[0]), ops.paged_decode_attention(kv, q, 640, ws=ws[1]))
+        jobs.append((run, [x.clone() for x in run(ws=ws)], torch.cuda.Stream()))
+
+    def at_once(calls):
+        torch.cuda.synchronize()
+        outs = []
+        for call, (_, _, stream) in zip(calls, jobs):
+            with torch.cuda.stream(stream):
+                for _ in range(4):
+                    out = call()
+                outs.append(out)
+        torch.cuda.synchronize()
+        for out, job in zip(outs, jobs):
+            for a, b in zip(out, job[1]):
+                assert torch.equal(a, b)
+    graphs, outs = [], []
+    for run, _, _ in jobs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run())
+    at_once([run for run, _, _ in jobs])
+    at_once([lambda graph=graph, out=out: (graph.replay(), out)[1] for graph, out in zip(graphs, outs)])
+    at_once([run for run, _, _ in jobs])
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals(cuda):
     from transformer_surgeon_b200 import ops
@@ -753,3 +792,49 @@ def test_refusals(cuda):
         ops.BeamReorder([kv])                                     # rows without pages of their own
     with pytest.raises(ValueError):
         ops.BeamReorder([other])(torch.zeros(2, dtype=torch.int64, device=cuda))
+
+
+@pytest.mark.parametrize("fmt", ["fp8_page", "int8"])
+def test_refusals_of_shared_memory_and_of_other_shapes(cuda, fmt):
+    """Expanded tensors (a stride of 0, which the C entries take for "dense"), tensors of another type or shape, more sequences than the cache has."""
+    from transformer_surgeon_b200 import ops
+    for logits, scores in ((torch.zeros(1, 50, device=cuda).expand(4, 50), torch.zeros(2, 2, device=cuda)),
+                           (torch.zeros(1, 1, 50, device=cuda).expand(2, 2, 50), torch.zeros(2, 2, device=cuda))):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.beam_select(logits, scores)
+    table = torch.arange(6, dtype=torch.int32, device=cuda).reshape(3, 2)
+    kv = ops.PagedKV(fmt, 6, 2, 64, table, torch.full((3,), 5, dtype=torch.int32, device=cuda), cuda)
+    rope = rope_tables(64, 32, cuda)
+    x = torch.zeros(3, 2, 2, 64, device=cuda)
+    for bad in (x[:1].expand(3, 2, 2, 64)[:, :1], x[:, :1].expand(3, 2, 2, 64), x[:1, :1].expand(3, 2, 2, 64)):
+        for call in (lambda: kv.append(bad, bad), lambda: kv.rope_append(bad, x[:, :bad.shape[1]], x[:, :bad.shape[1]], rope)):
+            with pytest.raises(ValueError):
+                call()
+    for call in (lambda: kv.append(x, x.bfloat16()), lambda: kv.append(x, x[:, :1]), lambda: kv.append(x[:, :, :1], x[:, :, :1]),
+                 lambda: kv.append(x.repeat(2, 1, 1, 1), x.repeat(2, 1, 1, 1)), lambda: kv.append(x, x, seq_lens=kv.seq_lens[:2]),
+                 lambda: kv.rope_append(x.bfloat16(), x, x, rope), lambda: kv.rope_append(x[:2], x, x, rope),
+                 lambda: ops.paged_decode_attention(kv, x[:1, 0].expand(3, 2, 64), 32), lambda: ops.paged_decode_attention(kv, x.view(6, 2, 64), 32),
+                 lambda: ops.paged_decode_attention(kv, x.view(3, 2, 128), 32)):
+        with pytest.raises(ValueError):
+            call()
+    ops.paged_decode_attention(kv, x[:, 0], 32)
+    torch.cuda.synchronize()
+
+
+def test_prompt_of_32_bits_with_overlapping_launches(cuda):
+    """The attention of a prompt chunk behind the append that wrote its pages, the engine's way (lengths and tables made once for all layers)."""
+    from transformer_surgeon_b200 import ops
+    outs = []
+    for pdl in (False, True):
+        kv = make_kv(2, 40, 2, 64, cuda, lens=[600, 600])
+        x = torch.randn(3, 2, 600, 2, 64, generator=torch.Generator().manual_seed(5)).to(cuda)
+        sequences, zeros = ops.query_sequences(kv, 2, 600, 600), torch.zeros_like(kv.seq_lens)
+        torch.cuda.synchronize()
+        old = ops.set_pdl(pdl)
+        try:
+            kv.append(x[1], x[2], seq_lens=zeros)
+            outs.append(ops.prefill_attention(kv, x[0].contiguous(), 600, sequences=sequences))
+            torch.cuda.synchronize()
+        finally:
+            ops.set_pdl(old)
+    assert torch.equal(outs[0], outs[1])

@@ -15,6 +15,7 @@ from ._lib import F32, BF16, KV_INT8, KV_FP8, KV_NVFP4, KV_F32, KV_BF16, KV_FP8_
 from ._lib import Tsb200Error  # noqa: F401  (re-exported)
 
 ATTN_STATUS_OFFSET = 16380      # byte offset of the status word inside an attention workspace (last int of the counter block)
+COUNTER_BYTES = 16384           # that block
 KV_FORMATS = {"int8": KV_INT8, "fp8": KV_FP8, "nvfp4": KV_NVFP4, "fp32": KV_F32, "bf16": KV_BF16, "fp8_page": KV_FP8_PAGE}
 PAGE = 16
 
@@ -67,13 +68,18 @@ def _token_strided(t, name):
     B, T, h, d = t.shape
     if t.numel() == 0:
         return h * d
-    if t.stride(3) != 1 or (h > 1 and t.stride(2) != d):     # the stride of a size-1 dimension is arbitrary
+    sb, st, sh, sd = t.stride()
+    if sd != 1 or (h > 1 and sh != d):                       # the stride of a size-1 dimension is arbitrary
         raise ValueError(f"{name}: the (heads, d) block of a token must be dense")
     if T == 1:                       # decode: one token per sequence, spaced by the batch stride
-        return t.stride(0) if B > 1 else h * d
-    if B > 1 and t.stride(0) != T * t.stride(1):
+        stride = sb if B > 1 else h * d
+    elif B > 1 and sb != T * st:
         raise ValueError(f"{name}: tokens must be evenly strided across the batch")
-    return t.stride(1)
+    else:
+        stride = st
+    if stride == 0:                  # the kernels take 0 for "dense"
+        raise ValueError(f"{name}: tokens must not share memory (an expanded tensor)")
+    return stride
 
 
 # ---------------------------------------------------------------- weights ----------
@@ -235,6 +241,16 @@ def workspace(device, nbytes, kind="linear"):
         buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)   # status word / counters start at 0
         _workspaces[key] = buf
     return buf
+
+
+def _scratch(device, nbytes, kind, head=0):
+    """Scratch of a call that was given none: the current stream's own, or, while it is captured, the graph's own, whose first `head` bytes every
+    replay clears.  So calls on two streams, and two graphs, never share any."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(max(nbytes, COUNTER_BYTES), dtype=torch.uint8, device=device)
+        ws[:head].zero_()
+        return ws
+    return workspace(device, nbytes, (kind, _stream()))
 
 
 class PackedLinear:
@@ -480,11 +496,17 @@ class PagedKV:
         self.v_scale.copy_(torch.as_tensor(v_scale, dtype=torch.float32).expand_as(self.v_scale))
         self.fp8_scales_set = True
 
-    def desc(self, seq_lens=None):
+    def desc(self, seq_lens=None, rows=0):
+        """rows: sequences of the call."""
         # rebuilt on every call: block_table / seq_lens tensors may have been swapped
         seq = self.seq_lens if seq_lens is None else seq_lens
+        table_rows, width = self.block_table.shape
+        if rows > table_rows or rows > seq.numel():
+            raise ValueError(f"{rows} sequences, but the cache has {table_rows} and seq_lens {seq.numel()}")
+        if self.fmt == KV_FP8_PAGE and self.k_pool.get_device() != _current_device():
+            _here(_cuda(self.k_pool, "the cache"), "the cache")
         return KVDesc(self.fmt, self.hkv, self.head_dim, self.flags, self.num_pages, self.k_pool.data_ptr(),
-                      self.v_pool.data_ptr(), self.block_table.data_ptr(), self.block_table.shape[1],
+                      self.v_pool.data_ptr(), self.block_table.data_ptr(), width,
                       seq.data_ptr(), 0 if self.k_scale is None else self.k_scale.data_ptr(),
                       0 if self.v_scale is None else self.v_scale.data_ptr())
 
@@ -502,11 +524,16 @@ class PagedKV:
     def rope_append(self, q, k, v, rope, new_lens=None, seq_lens=None):
         """One launch: RoPE on q [B, T, H, d] in place, RoPE on k, quantize-and-append k, v."""
         lib = _lib.load()
-        B, T = k.shape[:2]
+        B, T, heads, size = shape = k.shape
         cos, sin = rope
-        d = self.desc(seq_lens)
+        d = self.desc(seq_lens, B)
+        if v.shape != shape or v.dtype != k.dtype or heads != self.hkv or size != self.head_dim:
+            raise ValueError(f"k and v must be [B, T, {self.hkv}, {self.head_dim}], of one type")
+        qB, qT, q_heads, q_size = q.shape
+        if qB != B or qT != T or q_size != size or q.dtype != k.dtype:
+            raise ValueError("q must have the sequences, tokens, head size and type of k")
         qs, ks, vs = _token_strided(q, "q"), _token_strided(k, "k"), _token_strided(v, "v")
-        check(lib.tsb200_rope_append(C.byref(d), _p(q), q.shape[2], qs, _p(k), _p(v), _dt(k), ks, vs, B, T,
+        check(lib.tsb200_rope_append(C.byref(d), _p(q), q_heads, qs, _p(k), _p(v), _dt(k), ks, vs, B, T,
                                      _p(new_lens), _p(cos), _p(sin), cos.shape[0], _stream()), "tsb200_rope_append")
 
     def append(self, k, v, new_lens=None, rope=None, seq_lens=None):
@@ -514,9 +541,11 @@ class PagedKV:
         seq_lens is NOT advanced (it is shared by all layers; advance it once per step).
         `seq_lens` overrides the tensor of write positions for this call."""
         lib = _lib.load()
-        B, T = k.shape[:2]
+        B, T, heads, size = shape = k.shape
         cos, sin = (None, None) if rope is None else rope
-        d = self.desc(seq_lens)
+        d = self.desc(seq_lens, B)
+        if v.shape != shape or v.dtype != k.dtype or heads != self.hkv or size != self.head_dim:
+            raise ValueError(f"k and v must be [B, T, {self.hkv}, {self.head_dim}], of one type")
         ks, vs = _token_strided(k, "k"), _token_strided(v, "v")
         check(lib.tsb200_kv_append(C.byref(d), _p(k), _p(v), _dt(k), ks, vs, B, T, _p(new_lens),
                                    _p(cos), _p(sin), 0 if cos is None else cos.shape[0], _stream()),
@@ -610,8 +639,8 @@ def prefill_attention(kv, q, L, sm_scale=None, out=None, status=None, seq_lens=N
         view = PagedKV.__new__(PagedKV)
         view.__dict__.update(kv.__dict__)
         view.block_table, view.seq_lens = table, lens
-        if sequences is None or kv.k_scale is not None:
-            view.flags = _lib.KV_FRESH       # tables or scales were made just now
+        if sequences is None or kv.k_scale is not None or kv.fmt == KV_FP8_PAGE:
+            view.flags = _lib.KV_FRESH       # tables or scales were made just now; pages, which this format's attention requests early, perhaps too
         if kv.k_scale is not None:
             view.k_scale, view.v_scale = kv.k_scale.repeat_interleave(T, dim=0).contiguous(), kv.v_scale.repeat_interleave(T, dim=0).contiguous()
         qq = q.reshape(B * T, H, d) if q.is_contiguous() else q.contiguous().reshape(B * T, H, d)
@@ -623,7 +652,7 @@ def prefill_attention(kv, q, L, sm_scale=None, out=None, status=None, seq_lens=N
     Lp = (L + 63) // 64 * 64
     kd = torch.empty((B, kv.hkv, L, d), dtype=torch.bfloat16, device=q.device)
     vt = torch.empty((B, kv.hkv, d, Lp), dtype=torch.bfloat16, device=q.device)
-    desc = kv.desc(seq_lens)
+    desc = kv.desc(seq_lens, B)
     check(lib.tsb200_kv_gather_heads(C.byref(desc), _p(kd), _p(vt), B, L, Lp, _stream()), "tsb200_kv_gather_heads")
     check(lib.tsb200_prefill_attn(_p(q), qs, _p(kd), _p(vt), _p(out), B, T, L, Lp, H, kv.hkv, d, float(sm_scale), _p(status),
                                   _stream()), "tsb200_prefill_attn")
@@ -642,18 +671,25 @@ def paged_decode_attention(kv, q, max_seq_len, sm_scale=None, out=None, ws=None,
     if not q.is_cuda:
         raise ValueError("q must be a CUDA tensor (this library has no CPU path)")
     B, H, d = q.shape
-    if q.numel() and (q.stride(2) != 1 or q.stride(1) != d):
+    qs, sh, sd = q.stride()
+    filled = q.numel()
+    if filled and (sd != 1 or sh != d):
         raise ValueError("q: heads/d must be dense")
-    qs = q.stride(0) if q.numel() else H * d
+    if d != kv.head_dim:
+        raise ValueError(f"q has heads of {d}, the cache of {kv.head_dim}")
+    if not filled or B == 1:
+        qs = H * d
+    if qs == 0 and filled:
+        raise ValueError("q: sequences must not share memory (an expanded tensor)")
     if out is None:
         out = torch.empty((B, H, d), dtype=q.dtype, device=q.device)
     nbytes = decode_attn_workspace_bytes(B, H, d, max_seq_len)
     if ws is None:
-        ws = workspace(q.device, nbytes, "attention")
+        ws = (_scratch if kv.fmt == KV_FP8_PAGE else workspace)(q.device, nbytes, "attention")
     if sm_scale is None:
         sm_scale = d ** -0.5
     fn = lib.tsb200_paged_decode_attn_simt if simt else lib.tsb200_paged_decode_attn
-    desc = kv.desc(seq_lens)
+    desc = kv.desc(seq_lens, B)
     check(fn(C.byref(desc), _p(q), _p(out), _dt(q), qs, B, H, float(sm_scale), int(max_seq_len), _p(ws), ws.numel(),
              _stream()), "tsb200_paged_decode_attn")
     return out
@@ -675,16 +711,22 @@ def beam_select(logits, scores, n=None, finished=None, pad_token=0, out=None, ws
     logits [B * K, V] (or [B, K, V]; rows may be evenly strided), scores fp32 [B, K] of the beams: value = score + log_softmax(logits).  Returns
     (values fp32, parents int32, tokens int64), [B, n] each, best first, ties to the lower beam and token; a parent is a row of the batch
     (b * K + beam), as BeamReorder takes it.  finished: bool [B, K]; such a beam goes on as pad_token at its own score only.  A beam of score
-    -inf, or with a NaN or +inf among its logits, has no continuations; places without any are filled at -inf.  ws: zero-filled once, of one stream."""
+    -inf, or with a NaN or +inf among its logits, has no continuations; places without any are filled at -inf.  ws: zero-filled once, for one call at a time;
+    by default each stream, and each captured call, has its own."""
     B, K = scores.shape
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor (this library has no CPU path)")
     _here(logits, "logits")
     if logits.dim() == 3:
         logits = logits.flatten(0, 1)
-    V = logits.shape[1]
-    if logits.shape[0] != B * K or (V > 1 and logits.stride(1) != 1):
+    rows, V = logits.shape
+    stride, step = logits.stride()
+    if rows != B * K or (V > 1 and step != 1):
         raise ValueError("logits must be [B * K, V] with unit stride in the last dimension")
+    if rows == 1:
+        stride = V
+    elif rows and stride < V:
+        raise ValueError("rows of logits must not share memory (an expanded tensor)")
     if scores.dtype != torch.float32:
         raise TypeError("scores must be float32")
     if finished is not None and (finished.dtype != torch.bool or finished.shape != scores.shape):
@@ -693,14 +735,14 @@ def beam_select(logits, scores, n=None, finished=None, pad_token=0, out=None, ws
     dt = _dt(logits)
     if out is None:
         out = scores.new_empty((B, n)), scores.new_empty((B, n), dtype=torch.int32), scores.new_empty((B, n), dtype=torch.int64)
-    elif any(o.shape != (B, n) or o.dtype != t for o, t in zip(out, (torch.float32, torch.int32, torch.int64))):
+    elif any(_cuda(o, "out").shape != (B, n) or o.dtype != t for o, t in zip(out, (torch.float32, torch.int32, torch.int64))):
         raise ValueError("out must be float32, int32 and int64 tensors [B, n]")
     if ws is None:
-        ws = workspace(logits.device, beam_select_workspace_bytes(B, K, V, logits.dtype, n), "beams")
+        ws = _scratch(logits.device, beam_select_workspace_bytes(B, K, V, logits.dtype, n), "beams", COUNTER_BYTES)
     values, parents, tokens = out
-    st = _lib.load().tsb200_beam_select(logits.data_ptr(), dt, logits.stride(0) if B * K > 1 else V, B, K, V, _cuda(scores, "scores").data_ptr(),
-                                        0 if finished is None else _cuda(finished, "finished").data_ptr(), int(pad_token), n, _cuda(values, "out").data_ptr(),
-                                        _cuda(parents, "out").data_ptr(), _cuda(tokens, "out").data_ptr(), ws.data_ptr(), ws.numel(), _stream())
+    st = _lib.load().tsb200_beam_select(logits.data_ptr(), dt, stride, B, K, V, _cuda(scores, "scores").data_ptr(),
+                                        0 if finished is None else _cuda(finished, "finished").data_ptr(), int(pad_token), n, values.data_ptr(),
+                                        parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel(), _stream())
     if st:
         check(st, "tsb200_beam_select")
     return out
