@@ -225,7 +225,7 @@ int tsb200_norm_mlp_gated(const tsb200_norm_desc* norm, const tsb200_linear_desc
  * appended to a page that holds others raise it where they need to (the older codes are then re-encoded) and never lower it; larger values
  * saturate.  Nothing beside the pages belongs to the cache, so that sequences can share pages and tokens come one by one.
  * Pools must be zero-filled once when allocated: slots of a page beyond the sequence length
- * are read (and masked) by the attention kernels and must hold finite bit patterns.
+ * are read (and masked) by the attention kernels and must hold finite bit patterns (fp8_page: the codes may be any).
  * ---------------------------------------------------------------------------------- */
 size_t tsb200_kv_record_bytes(int format, int head_dim);
 

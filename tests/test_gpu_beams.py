@@ -330,8 +330,29 @@ def test_attention_pages_of_extreme_scales(cuda):
     assert 0 < np.abs(ref).max() < 2.0 ** -30 and (np.abs(out - ref) <= tolerance("fp32", size, ref)).all()
 
 
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_leaves_out_what_is_behind_the_end(cuda, name, d):
+    """NaN and infinities cached behind the length that a call gives (tokens taken back) change no bit."""
+    from transformer_surgeon_b200 import ops
+    lens = [1, 2, 3, 5, 7, 15, 16, 17, 30, 0]
+    kv = make_kv(10, 4, 2, d, cuda, lens=lens)
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(10, 64, 2, d, generator=g) for _ in range(2))
+    q = torch.randn(10, 6, d, generator=g).to(DT[name]).to(cuda)
+    zeros, outs = torch.zeros_like(kv.seq_lens), []
+    for bad in (0.0, float("nan"), float("inf"), -float("inf")):
+        for b, n in enumerate(lens):
+            k[b, n:], v[b, n:] = bad, bad
+        kv.append(k.to(cuda), v.to(cuda), seq_lens=zeros)
+        outs.append(ops.paged_decode_attention(kv, q, 64))
+    assert torch.isfinite(outs[0]).all()
+    for out in outs[1:]:
+        assert torch.equal(out, outs[0])
+
+
 def test_attention_passes_nan_on_where_it_counts(cuda):
-    """A NaN among a head's cached values reaches that head's outputs and no other's; behind the sequence's end it reaches none."""
+    """A NaN among a head's cached values reaches that head's outputs and no other's."""
     from transformer_surgeon_b200 import ops
     kv = make_kv(2, 2, 2, 64, cuda, lens=[20, 20])
     x = torch.randn(2, 20, 2, 64, generator=torch.Generator().manual_seed(1)).to(cuda)
