@@ -21,12 +21,14 @@ constexpr int kSlots = 592, kEntries = 4 * kThreads, kMaxBeams = 256;
 constexpr int kCounters = 4096;         // sequences of a launch; their counters are the workspace's head
 constexpr int kMost = kMaxBest * (kMaxBest + 1);            // entries that can reach the merge's bound
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLeast = -1e37f;       // a row of nothing above this (the type's lowest value as a mask) counts the elements equal to its maximum
+// Up to this |x log2 e| a whole number R refers to its neighbours exactly, and x log2 e - R is rounded once.  Beyond (masks of -1e9 and the like, the
+// type's lowest value: x log2 e may be off by more than the range of exponents) sums refer to a logit m.
+constexpr float kFar = 4194304.f;
 
 struct Part {           // of a row's stretch
-  double sum;           // sum of 2^(x log2 e - R)
-  float R;              // -infinity: the stretch has no element above kLeast,
-  float m;              // its maximum is this and `sum` the number of elements that have it
+  double sum;           // sum of 2^(x log2 e - R), or, with R = -infinity, of 2^((x - m) log2 e); m = -infinity too: of nothing
+  float R;
+  float m;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -93,6 +95,16 @@ __device__ __forceinline__ float sum_of(uint64_t p) {
 }
 __device__ __forceinline__ double pow2(float e) {              // of a whole number from -1000 to 0, or less: zero
   return e < -1000.f ? 0.0 : __hiloint2double((1023 + (int)e) << 20, 0);
+}
+// What a sum of reference (R, m) is multiplied by to have the reference (Rn, mn), which is no lower.  m log2 e has 48 bits: exact.
+__device__ __noinline__ double to_reference(float R, float m, float Rn, float mn) {
+  const double a = R > -INFINITY ? (double)R : (double)m * (double)kLog2e, b = Rn > -INFINITY ? (double)Rn : (double)mn * (double)kLog2e;
+  return exp2(a - b);
+}
+// Of two references (R, -infinity) and (-infinity, m), the higher one.
+__device__ __forceinline__ void higher(float& R, float& m) {
+  if ((double)m * (double)kLog2e > (double)R) R = -INFINITY;
+  else m = -INFINITY;
 }
 
 // A value that the n-th largest of 64 groups' maxima reaches (x: this thread's maximum; a group: kThreads / 64 neighbours); -infinity where fewer than n
@@ -190,10 +202,10 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
         }
         Rn = warp_max(Rn);
         mn = warp_max(mn);
-        // to the greater R: by a power of two; parts without one count where no part has one, for the greatest m
-        auto scaled = [&](double sum, float Ri, float mi) {
-          return sum * (Rn > -INFINITY ? (Ri > -INFINITY ? (Rn < INFINITY ? pow2(Ri - Rn) : 1.0) : 0.0) : mi == mn ? 1.0 : 0.0);
-        };
+        // to the greatest R: by a power of two
+        const bool shifts = mn == -INFINITY;
+        if (!shifts) higher(Rn, mn);
+        auto scaled = [&](double sum, float Ri, float mi) { return sum * (shifts ? (Ri > -INFINITY ? pow2(Ri - Rn) : 0.0) : to_reference(Ri, mi, Rn, mn)); };
         all = i0 ? scaled(all, R, m) : 0.0;
 #pragma unroll
         for (int u = 0; u < U; ++u) all += scaled(__hiloint2double(raw[u].y, raw[u].x), __int_as_float(raw[u].z), __int_as_float(raw[u].w));
@@ -202,7 +214,7 @@ __device__ __forceinline__ void merge(MergeSmem& s, int* group, float* bound2, i
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-      if (R < INFINITY && all > 0.0) {
+      if (all > 0.0) {                                        // NaN where the row has one, or +infinity
         l = log(all) + (R > -INFINITY ? (double)R * (1.0 / (double)kLog2e) : 0.0);      // the log2 e that the sums were made with
         at = R > -INFINITY ? 0.f : m;
       }
@@ -366,7 +378,7 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
   };
   const uint64_t c = pair_of(kLog2e, kLog2e);
   uint64_t sums = pair_of(0.f, 0.f);
-  float R = -INFINITY, m = -INFINITY, bound = -INFINITY;       // m: with R = -infinity, the maximum, sums: how often
+  float R = -INFINITY, m = -INFINITY, bound = -INFINITY;       // one of R and m at most is above -infinity
   auto load_tile = [&](int t0, uint4 (&x)[kVec]) {
     if (t0 >= in0 && t0 + TILE <= min(v1, in1)) {
       const uint4* p = reinterpret_cast<const uint4*>(r.base) + t0 + tid;
@@ -393,13 +405,21 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
     if (t0 == v0) {
       float ref;
       bound = nth_group(most, n, s_group, s_bound, &ref);
-      if (ref > kLeast) R = ceilf(ref * kLog2e);
+      if (fabsf(ref) * kLog2e < kFar) R = ceilf(ref * kLog2e);
     }
-    if (most > kLeast && most * kLog2e > R + 100.f) {         // terms could leave fp32's range, or are the first above kLeast
+    if (most * kLog2e > R + 100.f) {                          // terms could leave fp32's range, or there is no R
       const float Rn = ceilf(most * kLog2e);
-      const float f = R == -INFINITY ? 0.f : ex2(R - Rn);
-      sums = pair_of(sum_of(sums) * f, 0.f);
-      R = Rn;
+      if (fabsf(Rn) <= kFar) {
+        if (most > m) {
+          sums = pair_of(sum_of(sums) * ex2(R > -INFINITY ? R - Rn : fmaf(m, kLog2e, -Rn)), 0.f);
+          R = Rn;
+          m = -INFINITY;
+        }
+      } else if (R > -INFINITY) {
+        sums = pair_of(sum_of(sums) * ex2(fmaf(most, -kLog2e, R)), 0.f);
+        m = most;
+        R = -INFINITY;
+      }
     }
     if (R > -INFINITY) {
       const uint64_t minus = pair_of(-R, -R);
@@ -414,9 +434,8 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const float y = to_f32<T>(e[i]);
-          if (y > m) { m = y; count = count * 0.f + 1.f; }     // what is not a number stays so
-          else if (y == m) count += y == -INFINITY ? 0.f : 1.f;
-          else if (!(y < m)) count = y;
+          if (y > m) { count = fmaf(count, ex2((m - y) * kLog2e), 1.f); m = y; }     // what is not a number stays so
+          else if (y != -INFINITY) count += ex2((y - m) * kLog2e);
         }
       }
       sums = pair_of(count, 0.f);
@@ -434,8 +453,12 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
 #pragma unroll
     for (int i = 0; i < kThreads / 32; ++i) { Rc = fmaxf(Rc, s_R[i]); mc = fmaxf(mc, s_m[i]); }
     double part = sum_of(sums);
-    if (Rc > -INFINITY) part *= R > -INFINITY ? (Rc < INFINITY ? pow2(R - Rc) : 1.0) : 0.0;
-    else part *= m == mc ? 1.0 : 0.0;
+    if (mc == -INFINITY) {
+      part *= R > -INFINITY ? pow2(R - Rc) : 0.0;
+    } else {
+      higher(Rc, mc);
+      part *= to_reference(R, m, Rc, mc);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
     if (lane == 0) s_sum[w] = part;
