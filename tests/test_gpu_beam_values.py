@@ -41,6 +41,19 @@ def check(logits, scores, n, atol, strict=False):
         assert near and not strict, (b, i, got[1][b], parents[b], got[2][b], tokens[b])
 
 
+# A dominating term, the last one of its thread: its argument x log2 e - R, at most 4 above, is rounded once (2^-23 bits: 8.3e-8 of the term), its exponential
+# is off by 2^-22 (2.4e-7), two additions follow or precede it (2^-24 each): 4.4e-7 of the sum, hence of the logarithm.
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+@pytest.mark.parametrize("above", [2, 12, 25, 45, 65, 200])
+def test_a_late_peak_keeps_its_bits(cuda, name, above):
+    K, V, n = 16, 40000, 32                        # two stretches a row, of several tiles each
+    g = torch.Generator().manual_seed(above)
+    x = torch.randn(K, V, generator=g)
+    x[:, -1] = 4 + above + torch.rand(K, generator=g)
+    scores = -0.25 * torch.arange(K).float()[None]
+    check(x.to(DT[name]).to(cuda), scores.to(cuda), n, 4.6e-7 if above > 2 else 5.5e-6)
+
+
 # Sums of at most 80 terms a thread, in fp32: 80 * 2^-24 and the above, 5.3e-6 at worst.
 @pytest.mark.parametrize("name", ["bf16", "fp32"])
 @pytest.mark.parametrize("shape", [(16, 40000, 32), (3, 40000, 8)])

@@ -2,7 +2,7 @@
 //   value[k, t] = score[k] + x[k, t] - logsumexp(x[k, :]),  the n largest, ties to the lowest k * V + t.
 //
 // One pass over the logits.  A CTA takes a stretch of one row, in vectors of 16 bytes: it sums 2^(x log2 e - R) (R: a whole number near the first
-// tile's maximum, so that sums are put together by exact shifts; fp32 over the few hundred terms of a thread, 64 bits from there on, since candidates of
+// tile's maximum, raised with the elements, so that sums are put together by exact shifts; fp32 over the few hundred terms of a thread, 64 bits from there on, since candidates of
 // different rows are told apart by less than 32 bits of a long sum hold) and notes vectors whose largest element can still be among the
 // stretch's n best.  What "can still be" means: the n-th largest of 64 group maxima of the first tile, a value that n elements reach.  At the end the n
 // best of the noted vectors hold the n best elements; those alone are looked at one by one.  More noted vectors than there is room for raise the
@@ -24,6 +24,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Up to this |x log2 e| a whole number R refers to its neighbours exactly, and x log2 e - R is rounded once.  Beyond (masks of -1e9 and the like, the
 // type's lowest value: x log2 e may be off by more than the range of exponents) sums refer to a logit m.
 constexpr float kFar = 4194304.f;
+// A thread's R follows its elements when they are this far above it: the sum's larger terms then have arguments of 4 at most, rounded to 2^-23 (an argument
+// near 100: 2^-18, eleven times the exponential's own error).
+constexpr float kAbove = 4.f;
 
 struct Part {           // of a row's stretch
   double sum;           // sum of 2^(x log2 e - R), or, with R = -infinity, of 2^((x - m) log2 e); m = -infinity too: of nothing
@@ -96,6 +99,7 @@ __device__ __forceinline__ float sum_of(uint64_t p) {
 __device__ __forceinline__ double pow2(float e) {              // of a whole number from -1000 to 0, or less: zero
   return e < -1000.f ? 0.0 : __hiloint2double((1023 + (int)e) << 20, 0);
 }
+__device__ __forceinline__ float pow2f(float e) { return e < -126.f ? 0.f : __int_as_float((127 + (int)e) << 23); }     // of a whole number up to 0
 // What a sum of reference (R, m) is multiplied by to have the reference (Rn, mn), which is no lower.  m log2 e has 48 bits: exact.
 __device__ __noinline__ double to_reference(float R, float m, float Rn, float mn) {
   const double a = R > -INFINITY ? (double)R : (double)m * (double)kLog2e, b = Rn > -INFINITY ? (double)Rn : (double)mn * (double)kLog2e;
@@ -407,11 +411,11 @@ beam_select_kernel(const T* __restrict__ logits, int64_t row_stride, int K, int 
       bound = nth_group(most, n, s_group, s_bound, &ref);
       if (fabsf(ref) * kLog2e < kFar) R = ceilf(ref * kLog2e);
     }
-    if (most * kLog2e > R + 100.f) {                          // terms could leave fp32's range, or there is no R
+    if (most * kLog2e > R + kAbove) {                         // or there is no R
       const float Rn = ceilf(most * kLog2e);
       if (fabsf(Rn) <= kFar) {
         if (most > m) {
-          sums = pair_of(sum_of(sums) * ex2(R > -INFINITY ? R - Rn : fmaf(m, kLog2e, -Rn)), 0.f);
+          sums = pair_of(sum_of(sums) * (R > -INFINITY ? pow2f(R - Rn) : ex2(fmaf(m, kLog2e, -Rn))), 0.f);
           R = Rn;
           m = -INFINITY;
         }
