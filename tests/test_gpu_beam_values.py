@@ -111,3 +111,19 @@ def test_infinite_and_missing_logits_beside_large_ones(cuda, name):
     dead[[0, 1, 7]] = float("nan")
     v, p, t = (o.cpu() for o in ops.beam_select(dead.to(DT[name]).to(cuda), scores.to(cuda), 5))
     assert (v == float("-inf")).all() and t[0].tolist() == [0, 1, 2, 3, 4]
+
+
+@pytest.mark.parametrize("K,n,kind", [(40, 32, "one value"), (256, 5, "one value"), (256, 32, "one value"), (40, 32, "some rows out"), (64, 32, "few values"),
+                                      (40, 32, "unequal scores"), (120, 9, "some rows out")])
+def test_merge_of_more_equal_entries_than_it_has_room_for(cuda, K, n, kind):
+    """K * n entries, all or most of them at the n-th value: the lowest k * V + t stay."""
+    V = 3000
+    x = torch.full((K, V), 1.5)
+    scores = torch.zeros(2, K)
+    if kind == "some rows out":
+        scores[:, 3::7] = float("-inf")
+    elif kind == "few values":
+        x = torch.randint(0, 2, (K, V), generator=torch.Generator().manual_seed(1)).float()[:1].expand(K, V)
+    elif kind == "unequal scores":
+        scores[0, ::2] = -1.0
+    check(torch.cat((x, x.flip(1))).contiguous().to(cuda), scores.to(cuda), n, 2e-6, strict=True)             # rows are equal bit by bit, so are their sums
