@@ -1,0 +1,71 @@
+"""Caches that the caller owns, before, during and after a beam search: binding others, starting anew, setting back."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def wrapper_for(batch, kv_format="fp32", max_len=64):
+    """A blocks-path wrapper over a tiny Llama of 512 tokens, and a model of the same weights."""
+    from tests.test_gpu_hf import tiny
+    from transformer_surgeon_b200 import blocks_path, surgeon
+    model = tiny("llama", torch.float32)
+    dec = surgeon.decoder_from_model(model, batch, max_len, kv_format)
+    decoder = blocks_path.PagedTransformerDecoder(dec.cfg, dec.layers, dec.final_norm, "paged_" + kv_format, max_len, batch, dec.device)
+    return blocks_path.LLMWrapper(model.get_input_embeddings(), decoder, model.lm_head)
+
+
+def prompt(B, T, seed=5):
+    return torch.randint(0, 512, (B, T), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def own(caches):
+    return len(set(caches.block_table.flatten().tolist())) == caches.block_table.numel()
+
+
+def close(a, b):
+    """fp32 sums in other orders: products of 128 and 256 terms in a few layers, 2^-12 of the largest is far above them and far below another token's."""
+    return (a - b).abs().max() <= 2.0 ** -12 * b.abs().max()
+
+
+@pytest.mark.parametrize("kv_format", ["fp32", "fp8_page"])
+def test_caches_leave_and_come_back_with_shared_pages(cuda, kv_format):
+    """prefill(beams=3) on caches A, a prompt on B, and A again: A's rows still hold their prompts."""
+    from transformer_surgeon_b200 import blocks_path
+    w = wrapper_for(6, kv_format)
+    a, b = (blocks_path.build_paged_caches(w.decoder) for _ in range(2))
+    ids = prompt(2, 37)
+    w._bind(a)
+    w.engine.prefill(ids, beams=3)
+    table, tokens = a.block_table.clone(), prompt(6, 1, 6)
+    assert not own(a)
+    w.prefill(prompt(6, 11, 7), b)
+    assert torch.equal(a.block_table, table) and own(b)
+    got = w(tokens, torch.tensor([37]), a)[0].clone()
+    straight = wrapper_for(6, kv_format)
+    c = blocks_path.build_paged_caches(straight.decoder)
+    straight._bind(c)
+    straight.engine.prefill(ids, beams=3)
+    assert torch.equal(got, straight(tokens, torch.tensor([37]), c)[0])
+    # a search on the caches that came back, and on those that left
+    for caches, engine in ((a, w), (b, w)):
+        engine._bind(caches)
+        seqs, scores = engine.engine.beam_search(ids, 8, 3)
+        straight._bind(c)
+        want = straight.engine.beam_search(ids, 8, 3)
+        assert torch.equal(seqs, want[0]) and torch.equal(scores, want[1])
+
+
+def test_another_engine_takes_over_shared_pages(cuda):
+    """Caches searched by one engine, bound to a second: it knows the rows' own pages too."""
+    from transformer_surgeon_b200 import blocks_path
+    w, other = wrapper_for(6), wrapper_for(6)
+    caches, ids = blocks_path.build_paged_caches(w.decoder), prompt(2, 37)
+    w._bind(caches)
+    want = w.engine.beam_search(ids, 8, 3)
+    assert not own(caches)
+    other._bind(caches)
+    got = other.engine.beam_search(ids, 8, 3)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    other.engine.reset()
+    assert own(caches) and int(caches.seq_lens.max()) == 0

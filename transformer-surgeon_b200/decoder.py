@@ -284,13 +284,14 @@ class CompressedDecoder:
 
     def reset(self):
         self.seq_lens.zero_()
-        if self._beams is not None:
-            self._beams.reset()
+        if self.kv:
+            self.kv[0].own_pages()
 
     def bind_caches(self, kv, block_table, seq_lens):
         """Run on caller-owned caches (the blocks-path contract: the caller owns the caches and threads them
         through every call, blocks/mha.py:608-612).  `kv`: one ops.PagedKV per layer sharing `block_table`
-        [B, pages] and `seq_lens` [B].  A captured graph holds the old addresses and is dropped."""
+        [B, pages] and `seq_lens` [B].  The caches bound before stay as they are, beams' shared pages among
+        them.  A captured graph holds the old addresses and is dropped."""
         c = self.cfg
         if len(kv) != c.num_layers or block_table.shape[0] != self.B or seq_lens.shape[0] != self.B:
             raise ValueError("caches do not match the engine (layers / batch)")
@@ -300,9 +301,7 @@ class CompressedDecoder:
                 raise ValueError("cache format / geometry differs from the engine's")
             if x.block_table is not block_table or x.seq_lens is not seq_lens:
                 raise ValueError("all layers must share one block table and one seq_lens tensor")
-        if self._beams is not None:
-            self._beams.reset()                  # the caches given back start with pages of their own
-            self._beams = None
+        self._beams = None                       # of the caches bound before
         self.kv, self.block_table, self.seq_lens = list(kv), block_table, seq_lens
         self.pages_per_seq = block_table.shape[1]
         self.max_seq_len = min(self.max_seq_len, self.pages_per_seq * ops.PAGE)

@@ -460,6 +460,7 @@ class PagedKV:
     """Pools + block table + lengths of ONE layer's quantized paged KV cache."""
 
     flags = 0          # _lib.KV_FRESH: see the header
+    pages = None       # RowPages of the block table, once a BeamReorder was built over the cache
 
     def __init__(self, fmt, num_pages, hkv, head_dim, block_table, seq_lens, device, k_scale=None, v_scale=None, k_pool=None, v_pool=None):
         """k_pool, v_pool: memory the caller has already (uint8 [num_pages, hkv, record bytes], of finite codes); allocated otherwise."""
@@ -495,6 +496,11 @@ class PagedKV:
         self.k_scale.copy_(torch.as_tensor(k_scale, dtype=torch.float32).expand_as(self.k_scale))
         self.v_scale.copy_(torch.as_tensor(v_scale, dtype=torch.float32).expand_as(self.v_scale))
         self.fp8_scales_set = True
+
+    def own_pages(self):
+        """Sequences start anew: every row its own pages again, whatever beams shared (for all layers of the block table)."""
+        if self.pages is not None and self.pages.table is self.block_table:
+            self.pages.restore()
 
     def desc(self, seq_lens=None, rows=0):
         """rows: sequences of the call."""
@@ -552,12 +558,31 @@ class PagedKV:
               "tsb200_kv_append")
 
 
+class RowPages:
+    """The pages that the rows of a block table own.  It belongs to the caches, and stays with them where engines and searches come and go."""
+
+    def __init__(self, table):
+        self.table, self.own, self.shared = table, None, False      # shared: a reordering ran since the rows had their own
+        self.take()
+
+    def take(self):
+        """The pages that the rows name now."""
+        ids = self.table.flatten().sort().values
+        if bool((ids[1:] == ids[:-1]).any()):
+            raise ValueError("every row of the block table must have pages of its own")
+        self.own = self.table.clone()
+
+    def restore(self):
+        self.table.copy_(self.own)
+        self.shared = False
+
+
 class BeamReorder:
     """Beam search's reordering of the caches of all layers: row r of the batch takes over the cached tokens of row parents[r].
 
-    kvs: one PagedKV per layer; they share one block table, whose rows name pages of their own when this is built.  Full pages are
-    shared through the block table, the open page is copied into the row's own: one launch, whatever the context.  Before a sequence is started
-    anew (seq_lens back to 0), `reset` gives every row its own pages again."""
+    kvs: one PagedKV per layer; they share one block table, whose rows name pages of their own when the first of these is built over them (`PagedKV.pages`
+    keeps which).  Full pages are shared through the block table, the open page is copied into the row's own: one launch, whatever the context.  Before
+    a sequence is started anew or set back (seq_lens below what a reordering saw), `reset` gives every row its own pages again."""
 
     def __init__(self, kvs):
         self.kvs = list(kvs)
@@ -571,10 +596,13 @@ class BeamReorder:
                 raise ValueError("all layers must share one block table")
         self.block_table, self.seq_lens = a.block_table, a.seq_lens
         _cuda(self.block_table, "block_table")
-        self.home = self.block_table.clone()
-        ids = self.home.flatten().sort().values
-        if bool((ids[1:] == ids[:-1]).any()):
-            raise ValueError("every row of the block table must have pages of its own")
+        self.pages = a.pages
+        if self.pages is None or self.pages.table is not self.block_table:
+            self.pages = RowPages(self.block_table)
+        elif not self.pages.shared:
+            self.pages.take()
+        for x in self.kvs:
+            x.pages = self.pages
         dev = self.block_table.device
         pools = [p for x in self.kvs for p in (x.k_pool, x.v_pool)]
         scales = [p for x in self.kvs for p in (x.k_scale, x.v_scale) if p is not None]
@@ -593,11 +621,12 @@ class BeamReorder:
         if _cuda(parents, "parents").dtype != torch.int32 or parents.numel() != rows or lens.dtype != torch.int32 or lens.numel() != rows:
             raise ValueError(f"parents and seq_lens must be int32 [{rows}]")
         n_pools, page_bytes, pages, n_scales, hkv = self._n
+        self.pages.shared = True
         check(_lib.load().tsb200_kv_reorder(_p(self._pools), n_pools, page_bytes, pages, _p(self._scales), n_scales, hkv, _p(self.block_table), width,
                                             _p(lens), _p(parents), rows, _stream()), "tsb200_kv_reorder")
 
     def reset(self):
-        self.block_table.copy_(self.home)
+        self.pages.restore()
 
 
 def kv_gather(kv, L, dtype=torch.bfloat16, seq_lens=None):
