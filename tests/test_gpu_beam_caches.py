@@ -69,3 +69,24 @@ def test_another_engine_takes_over_shared_pages(cuda):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     other.engine.reset()
     assert own(caches) and int(caches.seq_lens.max()) == 0
+
+
+@pytest.mark.parametrize("how", ["beam_search", "prefill"])
+def test_caches_reset_after_beams(cuda, how):
+    """PagedCaches.reset: every row its own pages again, so that tokens one by one are what they are on new caches."""
+    from transformer_surgeon_b200 import blocks_path
+    w = wrapper_for(6, "fp8_page")
+    caches, fresh = (blocks_path.build_paged_caches(w.decoder) for _ in range(2))
+    w._bind(caches)
+    if how == "beam_search":
+        w.engine.beam_search(prompt(2, 19), 20, 3)
+    else:
+        w.engine.prefill(prompt(2, 37), beams=3)
+    assert not own(caches)
+    caches.reset()
+    assert own(caches) and int(caches.seq_lens.max()) == 0        # before anything is appended: rows that share a page would write it at once
+    ids, got = prompt(6, 21, 8), []
+    for t in range(21):
+        got.append(w(ids[:, t], torch.tensor([t]), caches)[0].clone())
+    for t in range(21):
+        assert torch.equal(got[t], w(ids[:, t], torch.tensor([t]), fresh)[0])

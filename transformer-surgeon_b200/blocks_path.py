@@ -56,6 +56,8 @@ class PagedCaches:
 
     def reset(self):
         self.seq_lens.zero_()
+        for x in self.kv[:1]:                   # one block table for all layers
+            x.own_pages()
 
 
 class PagedTransformerDecoder:
