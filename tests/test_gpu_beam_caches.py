@@ -90,3 +90,23 @@ def test_caches_reset_after_beams(cuda, how):
         got.append(w(ids[:, t], torch.tensor([t]), caches)[0].clone())
     for t in range(21):
         assert torch.equal(got[t], w(ids[:, t], torch.tensor([t]), fresh)[0])
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_caches_hold_the_sequences_that_a_search_returns(cuda, captured):
+    """After beam_search, row by row: the next step goes on from the returned sequence, not from the beams ahead of the last selection."""
+    from tests.test_gpu_hf import tiny
+    from transformer_surgeon_b200 import surgeon
+    model = tiny("llama", torch.float32)
+    dec, alone = (surgeon.decoder_from_model(model, 6, 64, "fp32") for _ in range(2))
+    if captured:
+        dec.capture()
+    for T, new in ((19, 30), (19, 29), (16, 1), (37, 8), (9, 8)):
+        seqs, _ = dec.beam_search(prompt(2, T, T + new), new, 3)
+        rows = torch.cat((seqs.flatten(0, 1), prompt(6, 3, 9)), 1)
+        alone.reset()
+        for t in range(T + new - 1):
+            alone.step(rows[:, t])
+        assert torch.equal(dec.seq_lens, alone.seq_lens)
+        for t in range(T + new - 1, rows.shape[1]):
+            assert close(dec.step(rows[:, t]), alone.step(rows[:, t]))

@@ -405,7 +405,8 @@ class CompressedDecoder:
         """Beam search over input_ids [B, T] on an engine built for B * num_beams sequences: every step keeps the num_beams best continuations
         of a sequence by their summed log probabilities, and the caches follow them (full pages are shared between beams).  With eos_token_id a
         beam that ends stays as it is, padded with pad_token_id (default: eos_token_id).  Returns (sequences int64 [B, num_beams, T + max_new_tokens],
-        scores fp32 [B, num_beams]), best first.  The prompts go through prefill(), once for all their beams."""
+        scores fp32 [B, num_beams]), best first.  The prompts go through prefill(), once for all their beams.  Row b * num_beams + k of the caches is left
+        with all tokens but the last of sequences[b, k]: step() with those goes on from there; before lengths are set back, reset()."""
         ids = input_ids.to(self.device)
         B, T = ids.shape
         K = int(num_beams)
@@ -432,8 +433,8 @@ class CompressedDecoder:
             new[:, i] = tokens
             if finished is not None:
                 finished = finished.view(-1).index_select(0, rows).logical_or_(tokens == eos_token_id).view(B, K)
+            self._beams(rows, self.seq_lens)                             # after the last step too: the caches hold what is returned
             if i + 1 < max_new_tokens:
-                self._beams(rows, self.seq_lens)
                 logits = self.step(tokens)
         self.check_status()
         return torch.cat((ids[:, None].expand(B, K, T), new.view(B, K, max_new_tokens)), dim=2), scores
