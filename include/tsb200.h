@@ -296,7 +296,8 @@ int tsb200_rope_append(const tsb200_kv_desc* kv, void* q, int q_heads, int64_t q
  * `n_pools` pools (device array of device pointers to uint8 [num_pages, page_bytes]: K and V of every layer; page_bytes = hkv * record bytes) that
  * share one block table.  Full pages become shared: block_table[r][0 .. seq_lens[r] / 16) is the parent's.  The entries from there on are the row's own
  * and do not change; the page at seq_lens[r] / 16, where it holds tokens, gets the parent's bytes.  So that no row ever writes a page of another one, a
- * block table starts with pages of its own for every row, and is put back to them before a sequence is started anew.
+ * block table starts with pages of its own for every row, and is put back to them before a sequence is started anew.  Nor may lengths be set back below
+ * seq_lens / 16 * 16 of a reordering: the pages there may be several rows' by then, and an append would write them for all.
  * A row whose parent is itself, is out of range, or has another length keeps what it has.  scales (may be NULL): device array of n_scales device
  * pointers to fp32 [rows, scale_width], whose rows follow their parents too.  parents may name a row several times.  rows <= 2048.
  * With tsb200_set_pdl on, the first append or attention after this call must be at least the second launch after it. */

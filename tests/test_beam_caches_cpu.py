@@ -26,3 +26,25 @@ def test_reset_gives_rows_their_own_pages():
     home = share(caches)
     caches.reset()
     assert torch.equal(caches.block_table, home) and not caches.seq_lens.any() and not caches.kv[0].pages.shared
+
+
+def test_a_step_that_sets_sequences_back_separates_their_pages():
+    """A position in the open page or behind it changes nothing; one below copies what rows share into their own pages."""
+    import types
+    from transformer_surgeon_b200 import blocks_path
+    caches = caches_on_cpu()
+    home = share(caches)
+    shared, before = caches.block_table.clone(), [p.clone() for x in caches.kv for p in (x.k_pool, x.v_pool)]
+    w = blocks_path.LLMWrapper.__new__(blocks_path.LLMWrapper)
+    w.engine = types.SimpleNamespace(device="cpu", B=3, cfg=types.SimpleNamespace(kv_format="fp8_page"), step=lambda tokens: torch.zeros(3, 5))
+    w.decoder, w.cache_impl, w._bound = types.SimpleNamespace(max_cache_len=64), caches.cache_impl, caches
+    for pos in (40, 41, 32):
+        w(torch.zeros(3, dtype=torch.int64), torch.tensor([pos]), caches)
+        assert torch.equal(caches.block_table, shared)
+    caches.seq_lens.fill_(40)
+    w(torch.zeros(3, dtype=torch.int64), torch.tensor([31]), caches)
+    assert torch.equal(caches.block_table, home) and not caches.kv[0].pages.shared and caches.seq_lens.tolist() == [31] * 3
+    for pool, old in zip([p for x in caches.kv for p in (x.k_pool, x.v_pool)], before):
+        for row in range(3):
+            for page in range(4):
+                assert torch.equal(pool[home[row, page]], old[shared[row, page]])

@@ -110,3 +110,38 @@ def test_caches_hold_the_sequences_that_a_search_returns(cuda, captured):
         assert torch.equal(dec.seq_lens, alone.seq_lens)
         for t in range(T + new - 1, rows.shape[1]):
             assert close(dec.step(rows[:, t]), alone.step(rows[:, t]))
+
+
+@pytest.mark.parametrize("pos", [0, 5, 16, 30, 47])
+def test_steps_set_back_after_a_search(cuda, pos):
+    """`forward` at any position after a beam search, which it accepts as the blocks path does: every row goes on from its own sequence's first tokens."""
+    from transformer_surgeon_b200 import blocks_path
+    w, B, K, T, new = wrapper_for(6), 2, 3, 19, 30
+    caches, fresh = (blocks_path.build_paged_caches(w.decoder) for _ in range(2))
+    w._bind(caches)
+    seqs, _ = w.engine.beam_search(prompt(B, T), new, K)
+    rows = seqs.flatten(0, 1)                                      # 48 of their 49 tokens are cached
+    after, got = prompt(6, 3, 9), []
+    for t in range(3):
+        got.append(w(after[:, t], torch.tensor([pos + t]), caches)[0].clone())
+    assert own(caches) or pos >= 48 // 16 * 16
+    for t in range(pos):
+        w(rows[:, t], torch.tensor([t]), fresh)
+    for t in range(3):
+        assert close(got[t], w(after[:, t], torch.tensor([pos + t]), fresh)[0])
+
+
+def test_steps_that_go_on_after_a_search(cuda):
+    """Positions behind the search: the pages stay shared, and every row goes on from its whole sequence."""
+    from transformer_surgeon_b200 import blocks_path
+    w = wrapper_for(6)
+    caches, fresh = (blocks_path.build_paged_caches(w.decoder) for _ in range(2))
+    w._bind(caches)
+    seqs, _ = w.engine.beam_search(prompt(2, 37), 8, 3)
+    rows, got = torch.cat((seqs.flatten(0, 1), prompt(6, 6, 9)), 1), []
+    for t in range(44, rows.shape[1]):
+        got.append(w(rows[:, t], torch.tensor([t]), caches)[0].clone())
+    assert not own(caches)
+    for t in range(rows.shape[1]):
+        logits = w(rows[:, t], torch.tensor([t]), fresh)[0]
+        assert t < 44 or close(got[t - 44], logits)

@@ -187,6 +187,9 @@ class LLMWrapper:
             raise ValueError("paged_fp8: scales are unset - feed the prompt with LLMWrapper.prefill, or pass "
                              "fp8_scales to build_paged_caches")
         pos = torch.clamp(pos_id_tensor.reshape(-1).to(eng.device), 0, self.decoder.max_cache_len - 1).to(torch.int32)
+        pages = caches.kv[0].pages
+        if pages is not None and pages.shared and int(pos.min()) // ops.PAGE < int(caches.seq_lens.max()) // ops.PAGE:
+            pages.separate(caches.kv)                # set back behind a beam search: into pages that rows may share
         caches.seq_lens.copy_(pos.expand_as(caches.seq_lens))        # the step appends at seq_lens, then attends over seq_lens + 1
         logits = eng.step(input_ids.reshape(-1).to(eng.device))
         return (logits[0] if eng.B == 1 else logits), caches

@@ -563,6 +563,7 @@ class RowPages:
 
     def __init__(self, table):
         self.table, self.own, self.shared = table, None, False      # shared: a reordering ran since the rows had their own
+        self.replayed = False                                       # one was captured: it may run again at any time
         self.take()
 
     def take(self):
@@ -574,7 +575,18 @@ class RowPages:
 
     def restore(self):
         self.table.copy_(self.own)
-        self.shared = False
+        self.shared = self.replayed
+
+    def separate(self, kvs):
+        """Every row its own pages, with the bytes of those that it shares copied into them (one host read): it may then be set back to any token."""
+        to, source = self.own.flatten().long(), self.table.flatten().long()
+        pages = kvs[0].num_pages
+        at = ((to != source) & (to >= 0) & (to < pages) & (source >= 0) & (source < pages)).nonzero()[:, 0]
+        to, source = to[at], source[at]
+        for x in kvs:
+            for pool in (x.k_pool, x.v_pool):
+                pool[to] = pool[source]              # all are read before any is written
+        self.restore()
 
 
 class BeamReorder:
@@ -622,6 +634,7 @@ class BeamReorder:
             raise ValueError(f"parents and seq_lens must be int32 [{rows}]")
         n_pools, page_bytes, pages, n_scales, hkv = self._n
         self.pages.shared = True
+        self.pages.replayed = self.pages.replayed or torch.cuda.is_current_stream_capturing()
         check(_lib.load().tsb200_kv_reorder(_p(self._pools), n_pools, page_bytes, pages, _p(self._scales), n_scales, hkv, _p(self.block_table), width,
                                             _p(lens), _p(parents), rows, _stream()), "tsb200_kv_reorder")
 
