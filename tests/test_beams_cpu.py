@@ -33,3 +33,24 @@ def test_refusals_before_a_launch():
 def test_cache_vocabulary():
     from transformer_surgeon_b200 import blocks_path
     assert blocks_path.kv_format_of("paged_fp8_page") == "fp8_page"
+
+
+def test_searches_that_selection_or_reordering_refuses_end_before_the_prompt():
+    import types
+    from transformer_surgeon_b200.decoder import CompressedDecoder
+
+    def engine(rows):
+        dec = CompressedDecoder.__new__(CompressedDecoder)
+        dec.device, dec.B, dec.greedy_head, dec.max_seq_len, dec.cfg = "cpu", rows, False, 64, types.SimpleNamespace(vocab=100)
+
+        def prefill(ids, beams):
+            raise AssertionError("the prompt ran")
+        dec.prefill = prefill
+        return dec
+    for rows, prompts, beams, kw in ((33, 1, 33, {}), (2080, 65, 32, {}), (4, 1, 4, dict(eos_token_id=7, pad_token_id=100)), (4, 1, 4, dict(eos_token_id=7, pad_token_id=-1)),
+                                     (4, 1, 4, dict(eos_token_id=-1)), (4, 1, 3, {}), (4, 1, 0, {})):
+        with pytest.raises(ValueError):
+            engine(rows).beam_search(torch.zeros(prompts, 5, dtype=torch.int64), 5, beams, **kw)
+    for rows, prompts, beams, kw in ((32, 1, 32, {}), (2048, 64, 32, {}), (4, 1, 4, dict(eos_token_id=7, pad_token_id=99)), (4, 1, 4, dict(pad_token_id=200))):
+        with pytest.raises(AssertionError, match="the prompt ran"):
+            engine(rows).beam_search(torch.zeros(prompts, 5, dtype=torch.int64), 5, beams, **kw)

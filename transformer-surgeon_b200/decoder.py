@@ -412,11 +412,15 @@ class CompressedDecoder:
         K = int(num_beams)
         if K < 1 or B * K != self.B:
             raise ValueError(f"engine was built for {self.B} sequences, beam search needs {B} x {K}")
+        if K > ops.BEAM_BEST or self.B > ops.REORDER_ROWS:
+            raise ValueError(f"beam search takes up to {ops.BEAM_BEST} beams and {ops.REORDER_ROWS} rows")
         if self.greedy_head:
             raise ValueError("beam search needs the step's logits: set greedy_head = False before capture()")
         if max_new_tokens < 1 or T + max_new_tokens - 1 > self.max_seq_len:
             raise ValueError("prompt and new tokens do not fit the engine")
         pad = eos_token_id if pad_token_id is None else pad_token_id
+        if eos_token_id is not None and not 0 <= pad < self.cfg.vocab:
+            raise ValueError(f"pad_token_id {pad} is not a token")
         logits = self.prefill(ids, beams=K)
         if self._beams is None:                                          # one beam
             self._beams = ops.BeamReorder(self.kv)

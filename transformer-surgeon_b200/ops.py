@@ -18,6 +18,7 @@ ATTN_STATUS_OFFSET = 16380      # byte offset of the status word inside an atten
 COUNTER_BYTES = 16384           # that block
 KV_FORMATS = {"int8": KV_INT8, "fp8": KV_FP8, "nvfp4": KV_NVFP4, "fp32": KV_F32, "bf16": KV_BF16, "fp8_page": KV_FP8_PAGE}
 PAGE = 16
+BEAM_BEST, REORDER_ROWS = 32, 2048      # continuations that a selection takes of a sequence, rows that a reordering moves
 
 
 def set_pdl(enabled):
