@@ -61,6 +61,14 @@ def _here(t, name):
     return t
 
 
+def _all_here(what, *tensors):
+    """The call goes to the current device's current stream: every tensor that it is given (None passed over) must be there."""
+    here = _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
+
+
 def _token_strided(t, name):
     """t [B, T, heads, d] whose (heads, d) block is dense and whose tokens are evenly spaced
     (e.g. a column slice of a fused projection output).  Returns the token stride in elements."""
@@ -539,6 +547,8 @@ class PagedKV:
         qB, qT, q_heads, q_size = q.shape
         if qB != B or qT != T or q_size != size or q.dtype != k.dtype:
             raise ValueError("q must have the sequences, tokens, head size and type of k")
+        if self.fmt == KV_FP8_PAGE:
+            _all_here("rope_append", q, k, v, cos, sin, new_lens, seq_lens)
         qs, ks, vs = _token_strided(q, "q"), _token_strided(k, "k"), _token_strided(v, "v")
         check(lib.tsb200_rope_append(C.byref(d), _p(q), q_heads, qs, _p(k), _p(v), _dt(k), ks, vs, B, T,
                                      _p(new_lens), _p(cos), _p(sin), cos.shape[0], _stream()), "tsb200_rope_append")
@@ -553,6 +563,8 @@ class PagedKV:
         d = self.desc(seq_lens, B)
         if v.shape != shape or v.dtype != k.dtype or heads != self.hkv or size != self.head_dim:
             raise ValueError(f"k and v must be [B, T, {self.hkv}, {self.head_dim}], of one type")
+        if self.fmt == KV_FP8_PAGE:
+            _all_here("append", k, v, cos, sin, new_lens, seq_lens)
         ks, vs = _token_strided(k, "k"), _token_strided(v, "v")
         check(lib.tsb200_kv_append(C.byref(d), _p(k), _p(v), _dt(k), ks, vs, B, T, _p(new_lens),
                                    _p(cos), _p(sin), 0 if cos is None else cos.shape[0], _stream()),
@@ -614,13 +626,14 @@ class BeamReorder:
             self.pages = RowPages(self.block_table)
         elif not self.pages.shared:
             self.pages.take()
-        for x in self.kvs:
-            x.pages = self.pages
         dev = self.block_table.device
         pools = [p for x in self.kvs for p in (x.k_pool, x.v_pool)]
         scales = [p for x in self.kvs for p in (x.k_scale, x.v_scale) if p is not None]
-        for p in scales:
-            _cuda(p, "scale")
+        for p in pools + scales:
+            if _cuda(p, "pool or scale").get_device() != self.block_table.get_device():
+                raise ValueError("pools, scales and block table must be on one device")
+        for x in self.kvs:
+            x.pages = self.pages
         self._held = pools + scales                      # their addresses are what the next two hold
         self._pools = torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64, device=dev)
         self._scales = torch.tensor([p.data_ptr() for p in scales], dtype=torch.int64, device=dev) if scales else None
@@ -631,6 +644,7 @@ class BeamReorder:
         row, where that is not the first layer's tensor."""
         rows, width = _here(self.block_table, "block_table").shape
         lens = self.seq_lens if seq_lens is None else _cuda(seq_lens, "seq_lens")
+        _all_here("reordering", parents, lens)
         if _cuda(parents, "parents").dtype != torch.int32 or parents.numel() != rows or lens.dtype != torch.int32 or lens.numel() != rows:
             raise ValueError(f"parents and seq_lens must be int32 [{rows}]")
         n_pools, page_bytes, pages, n_scales, hkv = self._n
@@ -724,6 +738,8 @@ def paged_decode_attention(kv, q, max_seq_len, sm_scale=None, out=None, ws=None,
         qs = H * d
     if qs == 0 and filled:
         raise ValueError("q: sequences must not share memory (an expanded tensor)")
+    if kv.fmt == KV_FP8_PAGE:
+        _all_here("paged_decode_attention", q, out, ws, seq_lens)
     if out is None:
         out = torch.empty((B, H, d), dtype=q.dtype, device=q.device)
     nbytes = decode_attn_workspace_bytes(B, H, d, max_seq_len)
@@ -782,7 +798,10 @@ def beam_select(logits, scores, n=None, finished=None, pad_token=0, out=None, ws
         raise ValueError("out must be float32, int32 and int64 tensors [B, n]")
     if ws is None:
         ws = _scratch(logits.device, beam_select_workspace_bytes(B, K, V, logits.dtype, n), "beams", COUNTER_BYTES)
+    elif ws.dtype != torch.uint8 or not ws.is_contiguous():
+        raise ValueError("ws must be contiguous uint8")
     values, parents, tokens = out
+    _all_here("beam_select", scores, finished, values, parents, tokens, ws)
     st = _lib.load().tsb200_beam_select(logits.data_ptr(), dt, stride, B, K, V, _cuda(scores, "scores").data_ptr(),
                                         0 if finished is None else _cuda(finished, "finished").data_ptr(), int(pad_token), n, values.data_ptr(),
                                         parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel(), _stream())
