@@ -622,6 +622,18 @@ int launch(tsb200_kv_desc kv, const T* q, PageArgs a, int64_t B, float* ws, T* o
   return TSB200_OK;
 }
 
+// Whole sequences, if the most pages that a warp then gets are not many more than in equal ranges: the parts of cut ones cost a launch, about as long as
+// a warp takes for five pages (whole / cut, us: 58 sequences x 575 tokens, 8 kv heads, 3 pages more: 19.1 / 21.3; 68 x 2076, 4 heads, 3: 30.7 / 32.6; 4 x 519,
+// 2 heads, 6: 8.1 / 7.4; 92 x 1660, 2 heads, 8: 22.0 / 18.7; 5 x 1491, 2 heads, 16: 17.7 / 8.5; two chunks of fp32 heads: 40 x 600, 14 / 2, 4: 9.4 / 11.0;
+// 74 x 1500, 14 / 2, 1: 16.9 / 17.7; 64 x 2080, 28 / 4, 7: 46.2 / 45.3; 50 x 900, 28 / 4, 8: 24.4 / 23.4).  Lengths are known to the device alone: all count
+// as the longest.  Where the others are far shorter, whole is the wrong choice (37 x 4096 at most, 8 heads, one of them that long and the rest 100
+// tokens: 38.9 / 13.7; 32 x 2100, half to all: 26.5 / 27.5).  units: CTAs that share a range.
+bool whole_is_faster(int64_t B, int64_t units, int64_t pages) {
+  const int64_t ranges = units < kSlots ? kSlots / units : 1;
+  const int64_t whole = (B + ranges - 1) / ranges * ((pages + NW - 1) / NW), cut = B * pages / (ranges * NW);
+  return whole - cut <= 5;
+}
+
 template <typename T, int D>
 int launch_for(const tsb200_kv_desc& kv, const void* q, PageArgs a, int64_t B, float* ws, void* out, int* status, cudaStream_t st) {
   constexpr int HEADS = Cfg<T, D>::HEADS;
@@ -629,19 +641,16 @@ int launch_for(const tsb200_kv_desc& kv, const void* q, PageArgs a, int64_t B, f
   a.chunks = (g + HEADS - 1) / HEADS;
   a.heads = g < HEADS ? g : HEADS;
   if ((int64_t)kMaxRows * a.H > 0x7fffffffLL) return TSB200_ERR_UNSUPPORTED;
+  const int64_t pages = (a.max_seq_len + 15) / 16;
+  if (whole_is_faster(B, (int64_t)kv.hkv * a.chunks, pages)) a.S = 0;
+  if (a.S) {
+    a.per_min = (unsigned)((pages + a.S - 3) / (a.S - 2));
+    if (a.per_min < kMinPages) a.per_min = kMinPages;
+  }
   return launch<T, D>(kv, (const T*)q, a, B, ws, (T*)out, status, st);
 }
 
 }  // namespace
-
-// Whole sequences, if the most pages that a warp then gets are not many more than in equal ranges: the parts of cut ones cost a launch, about as long as
-// a warp takes for five pages (whole / cut, us: 58 sequences x 575 tokens, 8 kv heads, 3 pages more: 19.1 / 21.3; 68 x 2076, 4 heads, 3: 30.7 / 32.6; 4 x 519,
-// 2 heads, 6: 8.1 / 7.4; 92 x 1660, 2 heads, 8: 22.0 / 18.7; 5 x 1491, 2 heads, 16: 17.7 / 8.5).
-static bool whole_is_faster(int64_t B, int64_t units, int64_t pages) {
-  const int64_t ranges = units < kSlots ? kSlots / units : 1;
-  const int64_t whole = (B + ranges - 1) / ranges * ((pages + NW - 1) / NW), cut = B * pages / (ranges * NW);
-  return whole - cut <= 5;
-}
 
 int launch_attn_page(const tsb200_kv_desc& kv, const void* q, void* out, int dtype, int64_t qs, int64_t B, int H, float sm_scale, int64_t max_seq_len,
                      float* ws, size_t ws_bytes, int* status, cudaStream_t st) {
@@ -655,11 +664,6 @@ int launch_attn_page(const tsb200_kv_desc& kv, const void* q, void* out, int dty
   int64_t S = pages / 4 < 64 ? pages / 4 : 64;
   if (S > room) S = room;
   a.S = S < 3 ? 0 : (int)S;
-  if (whole_is_faster(B, kv.hkv, pages)) a.S = 0;
-  if (a.S) {
-    a.per_min = (unsigned)((pages + a.S - 3) / (a.S - 2));
-    if (a.per_min < kMinPages) a.per_min = kMinPages;
-  }
   if (dtype == TSB200_F32)
     return kv.head_dim == 64 ? launch_for<float, 64>(kv, q, a, B, ws, out, status, st) : launch_for<float, 128>(kv, q, a, B, ws, out, status, st);
   return kv.head_dim == 64 ? launch_for<__nv_bfloat16, 64>(kv, q, a, B, ws, out, status, st)
