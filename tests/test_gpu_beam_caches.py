@@ -145,3 +145,27 @@ def test_steps_that_go_on_after_a_search(cuda):
     for t in range(rows.shape[1]):
         logits = w(rows[:, t], torch.tensor([t]), fresh)[0]
         assert t < 44 or close(got[t - 44], logits)
+
+
+def test_a_captured_reordering_is_never_taken_for_the_last_one(cuda):
+    """A graph of a reordering, replayed behind a reset: a step that sets sequences back still finds that rows share pages."""
+    from transformer_surgeon_b200 import blocks_path, ops
+    w = wrapper_for(6)
+    caches = blocks_path.build_paged_caches(w.decoder)
+    reorder = ops.BeamReorder(caches.kv)
+    parents = torch.tensor([0, 0, 0, 3, 3, 3], dtype=torch.int32, device=cuda)
+    graph = torch.cuda.CUDAGraph()
+    reorder(parents)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        reorder(parents)
+    caches.reset()
+    ids = prompt(6, 37)
+    want = w.prefill(ids, caches)[0].clone()
+    graph.replay()
+    assert not own(caches)
+    got = w(ids[:, 10], torch.tensor([10]), caches)[0].clone()
+    assert own(caches)
+    w.prefill(ids[[0, 0, 0, 3, 3, 3]], caches)
+    assert close(got, w(ids[:, 10], torch.tensor([10]), caches)[0])
+    assert torch.equal(w.prefill(ids, caches)[0], want)
