@@ -223,7 +223,9 @@ int tsb200_norm_mlp_gated(const tsb200_norm_desc* norm, const tsb200_linear_desc
  *   V fp8_page : codes [d][16], then the same
  * fp8_page: the scale is 2^e, e the smallest integer with amax <= 448 * 2^e over the finite elements of the page's tokens, -40 <= e <= 40.  Tokens
  * appended to a page that holds others raise it where they need to (the older codes are then re-encoded) and never lower it; larger values
- * saturate.  Nothing beside the pages belongs to the cache, so that sequences can share pages and tokens come one by one.
+ * saturate.  Nothing beside the pages belongs to the cache, so that sequences can share pages and tokens come one by one.  Decode attention adds up
+ * softmax weight times page scale of V in 11 bits (bf16) or 22 (fp32) down to 2^-22 of a head's largest, and loses what is below 2^-33 (2^-44) of it: an
+ * element that is zero in the pages of large scale has that error from the others.
  * Pools must be zero-filled once when allocated: slots of a page beyond the sequence length
  * are read (and masked) by the attention kernels and must hold finite bit patterns (fp8_page: the codes may be any).
  * ---------------------------------------------------------------------------------- */

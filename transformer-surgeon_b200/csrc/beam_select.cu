@@ -9,8 +9,9 @@
 // bound, and the stretch is read once more; each such pass strictly raises it, and what is left does not depend on the order of the atomics.
 // The last CTA of a sequence to be done adds up the rows' sums, turns the sorted lists into values in 64 bits and merges them (as a second launch, chained to
 // the first, about as long on the device and 4 us more of the host's time a call).
-// Many rows: 32 x 8 beams of 152064 31 us, of which the bytes alone take 12, without exponentials 24.6, without what follows the noted vectors 26.3: the
-// exponential unit sets the loop's pace (tiles requested ahead into registers 31, into shared memory 34; the bound raised again after 2, 4, 8 tiles 32); few: the chain of steps behind the logits.
+// Many rows: 32 x 8 beams of 152064 30.9 us, of which the bytes alone take 12; without the merge 25.5, without all that is behind the loop 22.7, without
+// exponentials 27.7.  No unit is full (exponentials 47 %, issue slots 46 %, memory 29 %): a tile's loads, the wait for them and its arithmetic follow one
+// another in a CTA (tiles requested ahead into registers 31, into shared memory 34; the bound raised again after 2, 4, 8 tiles 32).  Few: the chain of steps behind the logits.
 #include "common.cuh"
 
 namespace tsb {

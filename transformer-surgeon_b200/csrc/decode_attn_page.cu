@@ -2,18 +2,21 @@
 //   out[h] = sum_t p_t V_t / sum_t p_t,  p_t = exp(sm_scale q_h . K_t),  K_t = 2^eK code, V_t = 2^eV code,  e per page.
 // The scale of V joins the exponent:
 //   w_t = 2^(s_t + eV - M + 8),  numerator sum w_t code_t,  denominator sum w_t 2^-eV   (s_t in bits; M is at most 6 below the largest s_t + eV so far),
-// so that pages of any scales share one accumulator and the maximum moves rarely.
+// so that pages of any scales share one accumulator and the maximum moves rarely.  The largest w of a head lies between 2^8 and 2^14; a w keeps the bits that
+// are said below down to 2^-14, 22 bits under it at least, and is nothing below 2^-25 (two terms: 2^-36).  So an element's error is that share of the head's largest
+// w code, also where the pages of large w hold zeros in that element.
 // Products run on warp-level f16 MMAs (m16n8k16), whose 16 rows are a page's tokens (elements of V) and whose 8 columns are query heads: 8 of bf16
 // (a query scaled by a power of two is an f16 number, weights keep 11 bits), 4 of fp32 in two f16 terms, code and rest * 2^11 (22 bits).  The
-// codes are widened to f16 pairs, one conversion for two; the e4m3 form of the MMA does the same in every instruction, to both operands: 850
-// instructions for two pages of 128, 300 here.  A word of four codes is a k-step of the first product and half a row of the second, with the
+// codes are widened to f16 pairs, one conversion for two; the e4m3 form of the MMA does the same in every instruction, to both operands: 425
+// instructions for a page of 128, 305 here.  A word of four codes is a k-step of the first product and half a row of the second, with the
 // tokens of both in the order that makes the transposed weights (movmatrix) the second one's operand.
 //
 // Work: the pages of all sequences in one row, cut into equal ranges, each for as many CTAs as there are kv heads, together as many as the device holds,
 // and each of those into equal ranges of its warps.  A warp streams its pages through a private ring (cp.async.bulk, K and V record) that does not
 // drain between sequences; a sequence that lies in one warp's range is done there, one that crosses warps is put together in shared memory
-// at the CTA's end, one that crosses ranges by a second launch (by the last of its CTAs: 5 us longer, one CTA then waits for every step of that alone).  So lengths of any mixture keep every SM busy to the end, and the heads of a page,
-// neighbours in memory, are read at about the same time (64 x 8192 tokens, 8 heads, pages in random order: 5.5 TB/s where they were not).
+// at the CTA's end, one that crosses ranges by a second launch (by the last of its CTAs: 5 us longer, one CTA then waits for every step of that alone).
+// So, where sequences are cut (whole_is_faster), lengths of any mixture keep every SM busy to the end, and the heads of a page, neighbours in memory, are read
+// at about the same time (64 x 8192 tokens, 8 heads, pages in random order: 5.5 TB/s where they were not).
 #include "tc_common.cuh"
 #include "decode_attn_common.cuh"
 #include "kv_page.cuh"
