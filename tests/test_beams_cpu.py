@@ -76,7 +76,7 @@ def test_tensors_of_another_device_are_refused(monkeypatch, where):
     from transformer_surgeon_b200 import ops
     monkeypatch.setattr(ops, "_current_device", lambda: 0)
     monkeypatch.setattr(ops, "_stream", lambda: 0)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(ops, "_capturing", lambda: False)
     launched = []
     lib = ops._lib.load()
 

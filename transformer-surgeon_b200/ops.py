@@ -26,7 +26,7 @@ def set_pdl(enabled):
     return bool(_lib.load().tsb200_set_pdl(int(bool(enabled))))
 
 
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_raw_stream, _current_device, _capturing = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice, torch._C._cuda_isCurrentStreamCapturing
 
 
 def _stream():
@@ -56,17 +56,9 @@ def _cuda(t, name):
 
 def _here(t, name):
     """t on the current device: the call goes to that device's current stream."""
-    if t.device.index != _current_device():
+    if t.get_device() != _current_device():
         raise ValueError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
     return t
-
-
-def _all_here(what, *tensors):
-    """The call goes to the current device's current stream: every tensor that it is given (None passed over) must be there."""
-    here = _current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
 
 
 def _token_strided(t, name):
@@ -255,7 +247,7 @@ def workspace(device, nbytes, kind="linear"):
 def _scratch(device, nbytes, kind, head=0):
     """Scratch of a call that was given none: the current stream's own, or, while it is captured, the graph's own, whose first `head` bytes every
     replay clears.  So calls on two streams, and two graphs, never share any."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         ws = torch.empty(max(nbytes, COUNTER_BYTES), dtype=torch.uint8, device=device)
         ws[:head].zero_()
         return ws
@@ -548,7 +540,10 @@ class PagedKV:
         if qB != B or qT != T or q_size != size or q.dtype != k.dtype:
             raise ValueError("q must have the sequences, tokens, head size and type of k")
         if self.fmt == KV_FP8_PAGE:
-            _all_here("rope_append", q, k, v, cos, sin, new_lens, seq_lens)
+            here = self.k_pool.get_device()                  # the current device: desc
+            if (q.get_device() != here or k.get_device() != here or v.get_device() != here or cos.get_device() != here or sin.get_device() != here or
+                    (new_lens is not None and new_lens.get_device() != here) or (seq_lens is not None and seq_lens.get_device() != here)):
+                raise ValueError(f"a tensor is on another device than the cache, cuda:{here}")
         qs, ks, vs = _token_strided(q, "q"), _token_strided(k, "k"), _token_strided(v, "v")
         check(lib.tsb200_rope_append(C.byref(d), _p(q), q_heads, qs, _p(k), _p(v), _dt(k), ks, vs, B, T,
                                      _p(new_lens), _p(cos), _p(sin), cos.shape[0], _stream()), "tsb200_rope_append")
@@ -564,7 +559,10 @@ class PagedKV:
         if v.shape != shape or v.dtype != k.dtype or heads != self.hkv or size != self.head_dim:
             raise ValueError(f"k and v must be [B, T, {self.hkv}, {self.head_dim}], of one type")
         if self.fmt == KV_FP8_PAGE:
-            _all_here("append", k, v, cos, sin, new_lens, seq_lens)
+            here = self.k_pool.get_device()
+            for t in (k, v, cos, sin, new_lens, seq_lens):
+                if t is not None and t.get_device() != here:
+                    raise ValueError(f"a tensor is on another device than the cache, cuda:{here}")
         ks, vs = _token_strided(k, "k"), _token_strided(v, "v")
         check(lib.tsb200_kv_append(C.byref(d), _p(k), _p(v), _dt(k), ks, vs, B, T, _p(new_lens),
                                    _p(cos), _p(sin), 0 if cos is None else cos.shape[0], _stream()),
@@ -642,16 +640,21 @@ class BeamReorder:
     def __call__(self, parents, seq_lens=None):
         """parents int32 [rows]; a row whose parent is itself, out of range or of another length keeps what it has.  seq_lens: tokens cached per
         row, where that is not the first layer's tensor."""
-        rows, width = _here(self.block_table, "block_table").shape
-        lens = self.seq_lens if seq_lens is None else _cuda(seq_lens, "seq_lens")
-        _all_here("reordering", parents, lens)
-        if _cuda(parents, "parents").dtype != torch.int32 or parents.numel() != rows or lens.dtype != torch.int32 or lens.numel() != rows:
+        table, here = self.block_table, _current_device()
+        rows, width = table.shape
+        lens = self.seq_lens if seq_lens is None else seq_lens
+        if table.get_device() != here or parents.get_device() != here or lens.get_device() != here:
+            raise ValueError(f"block table, parents and seq_lens must be on the current device, cuda:{here}")
+        if parents.dtype != torch.int32 or parents.numel() != rows or lens.dtype != torch.int32 or lens.numel() != rows:
             raise ValueError(f"parents and seq_lens must be int32 [{rows}]")
+        if not parents.is_contiguous() or not lens.is_contiguous():
+            raise ValueError("parents and seq_lens must be contiguous")
         n_pools, page_bytes, pages, n_scales, hkv = self._n
         self.pages.shared = True
-        self.pages.replayed = self.pages.replayed or torch.cuda.is_current_stream_capturing()
-        check(_lib.load().tsb200_kv_reorder(_p(self._pools), n_pools, page_bytes, pages, _p(self._scales), n_scales, hkv, _p(self.block_table), width,
-                                            _p(lens), _p(parents), rows, _stream()), "tsb200_kv_reorder")
+        if _capturing():
+            self.pages.replayed = True
+        check(_lib.load().tsb200_kv_reorder(_p(self._pools), n_pools, page_bytes, pages, _p(self._scales), n_scales, hkv, table.data_ptr(), width,
+                                            lens.data_ptr(), parents.data_ptr(), rows, _stream()), "tsb200_kv_reorder")
 
     def reset(self):
         self.pages.restore()
@@ -739,7 +742,10 @@ def paged_decode_attention(kv, q, max_seq_len, sm_scale=None, out=None, ws=None,
     if qs == 0 and filled:
         raise ValueError("q: sequences must not share memory (an expanded tensor)")
     if kv.fmt == KV_FP8_PAGE:
-        _all_here("paged_decode_attention", q, out, ws, seq_lens)
+        _here(q, "q")
+        for t, name in ((out, "out"), (ws, "ws"), (seq_lens, "seq_lens")):
+            if t is not None:
+                _here(t, name)
     if out is None:
         out = torch.empty((B, H, d), dtype=q.dtype, device=q.device)
     nbytes = decode_attn_workspace_bytes(B, H, d, max_seq_len)
@@ -775,7 +781,9 @@ def beam_select(logits, scores, n=None, finished=None, pad_token=0, out=None, ws
     B, K = scores.shape
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor (this library has no CPU path)")
-    _here(logits, "logits")
+    here = _current_device()
+    if logits.get_device() != here or scores.get_device() != here or (finished is not None and finished.get_device() != here):
+        raise ValueError(f"logits, scores and finished must be on the current device, cuda:{here}")
     if logits.dim() == 3:
         logits = logits.flatten(0, 1)
     rows, V = logits.shape
@@ -794,14 +802,13 @@ def beam_select(logits, scores, n=None, finished=None, pad_token=0, out=None, ws
     dt = _dt(logits)
     if out is None:
         out = scores.new_empty((B, n)), scores.new_empty((B, n), dtype=torch.int32), scores.new_empty((B, n), dtype=torch.int64)
-    elif any(_cuda(o, "out").shape != (B, n) or o.dtype != t for o, t in zip(out, (torch.float32, torch.int32, torch.int64))):
+    elif any(_here(_cuda(o, "out"), "out").shape != (B, n) or o.dtype != t for o, t in zip(out, (torch.float32, torch.int32, torch.int64))):
         raise ValueError("out must be float32, int32 and int64 tensors [B, n]")
     if ws is None:
         ws = _scratch(logits.device, beam_select_workspace_bytes(B, K, V, logits.dtype, n), "beams", COUNTER_BYTES)
-    elif ws.dtype != torch.uint8 or not ws.is_contiguous():
-        raise ValueError("ws must be contiguous uint8")
+    elif _here(_cuda(ws, "ws"), "ws").dtype != torch.uint8:
+        raise ValueError("ws must be uint8")
     values, parents, tokens = out
-    _all_here("beam_select", scores, finished, values, parents, tokens, ws)
     st = _lib.load().tsb200_beam_select(logits.data_ptr(), dt, stride, B, K, V, _cuda(scores, "scores").data_ptr(),
                                         0 if finished is None else _cuda(finished, "finished").data_ptr(), int(pad_token), n, values.data_ptr(),
                                         parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel(), _stream())
