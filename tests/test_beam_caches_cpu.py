@@ -48,3 +48,14 @@ def test_a_step_that_sets_sequences_back_separates_their_pages():
         for row in range(3):
             for page in range(4):
                 assert torch.equal(pool[home[row, page]], old[shared[row, page]])
+
+
+def test_reset_leaves_a_table_alone_that_no_beams_share():
+    """Pages handed out anew by the caller, after a search was over and put back: a reset does not take them away."""
+    caches = caches_on_cpu()
+    share(caches)
+    caches.reset()
+    mine = caches.block_table.flip(0).clone()
+    caches.block_table.copy_(mine)
+    caches.reset()
+    assert torch.equal(caches.block_table, mine)

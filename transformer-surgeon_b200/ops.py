@@ -499,8 +499,8 @@ class PagedKV:
         self.fp8_scales_set = True
 
     def own_pages(self):
-        """Sequences start anew: every row its own pages again, whatever beams shared (for all layers of the block table)."""
-        if self.pages is not None and self.pages.table is self.block_table:
+        """Sequences start anew: every row its own pages again, if beams shared any (for all layers of the block table)."""
+        if self.pages is not None and self.pages.shared and self.pages.table is self.block_table:
             self.pages.restore()
 
     def desc(self, seq_lens=None, rows=0):
